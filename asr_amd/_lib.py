@@ -20,7 +20,7 @@ CONV_TOEPLITZ = 1
 CONV_FFT = 2
 CONV_SCAN = 3
 NOALLOC_SCRATCH_BYTES = 8 << 20
-ABI_VERSION = 31
+ABI_VERSION = 32
 
 
 class Shape(ctypes.Structure):
@@ -260,6 +260,15 @@ def _load():
     lib.lmufft_backward_needs_gm_bf16.argtypes = [sp, ci, ci]
     lib.lmufft_dropout_epoch.restype = ci
     lib.lmufft_dropout_epoch.argtypes = [vp]
+    lib.lmufft_decay_workspace_bytes.restype = sz
+    lib.lmufft_decay_workspace_bytes.argtypes = [ci, i32, i32, i32, i32, i32, ci]
+    lib.lmufft_decay_attention.restype = ci
+    lib.lmufft_decay_attention.argtypes = [vp, vp, vp, ci] + [i64] * 6 + [vp, vp] + [i32] * 5 + [f32, vp, i64, i64, vp, vp, sz, vp]
+    lib.lmufft_decay_attention_bwd.restype = ci
+    lib.lmufft_decay_attention_bwd.argtypes = [vp, vp, vp, vp, ci] + [i64] * 8 + [vp, vp] + [i32] * 5 + [
+        f32, vp, vp, vp] + [i64] * 6 + [vp, sz, vp]
+    lib.lmufft_decay_attention_step.restype = ci
+    lib.lmufft_decay_attention_step.argtypes = [vp, vp, vp, ci, i64, i64, i64, vp, vp, i32, i32, i32, i32, f32, vp, i64, vp, vp]
     lib.lmufft_linear_wprep_bf16.restype = ci
     lib.lmufft_linear_wprep_bf16.argtypes = [vp, vp, i32, i32, i32, vp, vp, i64, vp, vp]
     lib.lmufft_linear_wprep_many_bf16.restype = ci
@@ -343,6 +352,10 @@ EXPORTS = (
     "lmufft_layernorm_dropout_bwd_relu",
     "lmufft_layernorm_param_sum_many",
     "lmufft_dropout_epoch",
+    "lmufft_decay_workspace_bytes",
+    "lmufft_decay_attention",
+    "lmufft_decay_attention_bwd",
+    "lmufft_decay_attention_step",
     "lmufft_linear_bf16",
     "lmufft_linear_ln_bf16",
     "lmufft_linear_wprep_bf16",

@@ -1,0 +1,217 @@
+// C entry points of the causal decay attention (kernels: decay_core.h), and its single-frame form.
+//
+// k_decay_step: S <- lambda S + k v^T, o = scale S^T q for one frame of each stream, the state updated in place.
+//   One workgroup per (stream, head): DV / 4 threads side by side own four columns each, the workgroup's rows of threads
+//   split the DK rows of the state; the partial sums over their rows meet in LDS.  Every element of the state is read and
+//   written once, 16 bytes a lane: bound by the states' traffic (8 DK DV bytes a stream and head) when there are many
+//   streams, by the launch when there are few.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "decay_core.h"
+
+namespace lmufft {
+
+constexpr int kDecayStepThreads = 256;
+
+template <class T, int DV>
+__global__ __launch_bounds__(kDecayStepThreads) void k_decay_step(const T* __restrict__ q, const T* __restrict__ k,
+                                                                  const T* __restrict__ v, long ldq, long ldk, long ldv,
+                                                                  const float* __restrict__ log_decay,
+                                                                  const int* __restrict__ active, int H, int DK,
+                                                                  float scale, T* __restrict__ out, long ldo,
+                                                                  float* __restrict__ state) {
+  constexpr int CV = DV / 4, RG = kDecayStepThreads / CV;  // threads across the columns; rows of threads
+  __shared__ __attribute__((aligned(16))) float part[RG * DV];
+  const int tid = threadIdx.x, c = (tid % CV) * 4, rg = tid / CV;
+  const int b = blockIdx.x / H, h = blockIdx.x - b * H;
+  T* const op = out + (long)b * ldo + (long)h * DV;
+  if (active && active[b] <= 0) {  // a silent stream: zeros, and its state stays as it is
+    if (tid < DV) op[tid] = (T)0.f;
+    return;
+  }
+  const T* const qp = q + (long)b * ldq + (long)h * DK;
+  const T* const kp = k + (long)b * ldk + (long)h * DK;
+  const T* const vp = v + (long)b * ldv + (long)h * DV + c;
+  const float lam = exp2f(log_decay[h] * 1.4426950408889634f);
+  dec_f4 vv;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) vv[e] = (float)vp[e];
+  dec_f4 o = dec_f4(0.f);
+  float* const sp = state + (long)blockIdx.x * DK * DV + c;
+#pragma unroll 4
+  for (int r = rg; r < DK; r += RG) {
+    dec_f4* const e = reinterpret_cast<dec_f4*>(sp + (long)r * DV);
+    const dec_f4 s = lam * *e + (float)kp[r] * vv;
+    *e = s;
+    o += (float)qp[r] * s;
+  }
+  *reinterpret_cast<dec_f4*>(&part[rg * DV + c]) = o;
+  __syncthreads();
+  if (tid < DV) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < RG; ++i) t += part[i * DV + tid];
+    op[tid] = (T)(t * scale);
+  }
+}
+
+static bool decay_width(int d) { return d == 32 || d == 64 || d == 128; }
+
+static int decay_check(const char* what, int dtype, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv) {
+  if (dtype != LMUFFT_F32 && dtype != LMUFFT_BF16) return set_error("%s: unknown dtype %d", what, dtype);
+  if (B < 0 || T < 0 || H <= 0) return set_error("%s: bad shape (B=%d T=%d H=%d)", what, B, T, H);
+  if (!decay_width(dk) || !decay_width(dv)) return set_error("%s: head widths %d, %d (supported: 32, 64, 128)", what, dk, dv);
+  if ((long)B * H > 0x7fffffffL || T > (1 << 26)) return set_error("%s: too large (B=%d T=%d H=%d)", what, B, T, H);
+  return 0;
+}
+
+// Segments an utterance's frames are split into: enough workgroups to fill the chip when there are few heads in all.
+// A split costs a second read of k and v and a launch.
+static int decay_segments(int dtype, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int* seg_len) {
+  const int chunk = dtype == LMUFFT_BF16 ? decay_chunk_bf16(dk, dv) : decay_chunk_f32(dk, dv);
+  const long heads = (long)B * H, chunks = std::max<long>(1, (T + (long)chunk - 1) / chunk);
+  long n = std::min<long>(std::min<long>(kDecayMaxSegments, 1024 / std::max<long>(1, heads)), chunks / 2);
+  n = std::max<long>(n, 1);
+  const long per = (chunks + n - 1) / n;
+  *seg_len = (int)(per * chunk);
+  return (int)((chunks + per - 1) / per);
+}
+
+// Rows of [B][T][H * width] tensors have to start on 16-byte boundaries (the kernels load 16 bytes a lane).
+static int decay_tensor(const char* what, const char* name, const void* p, int dtype, int64_t ld, int64_t bs, int32_t B,
+                        int32_t T, long width, bool written, DecayTensor* out) {
+  if (!p) return set_error("%s: `%s` is NULL", what, name);
+  const int64_t unit = dtype == LMUFFT_F32 ? 4 : 8;
+  if ((reinterpret_cast<uintptr_t>(p) & 15) || ld % unit || bs % unit)
+    return set_error("%s: rows of `%s` must start on 16-byte boundaries", what, name);
+  if (ld < 0 || bs < 0) return set_error("%s: `%s` has a negative stride", what, name);
+  if (written && ((T > 1 && ld < width) || (B > 1 && bs < (T - 1) * ld + width)))
+    return set_error("%s: rows of `%s` overlap", what, name);
+  out->p = p;
+  out->ld = ld;
+  out->bs = bs;
+  return 0;
+}
+
+static int decay_launch_any(int dtype, const DecayArgs& a, int roles, int dk, int dv, hipStream_t st) {
+  return dtype == LMUFFT_BF16 ? decay_launch_bf16(a, roles, dk, dv, st) : decay_launch_f32(a, roles, dk, dv, st);
+}
+
+}  // namespace lmufft
+
+using namespace lmufft;
+
+extern "C" size_t lmufft_decay_workspace_bytes(int dtype, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv,
+                                               int backward) {
+  if (decay_check("decay attention", dtype, B, T, H, dk, dv)) return 0;
+  int seg_len = 0;
+  const int n = decay_segments(dtype, B, T, H, dk, dv, &seg_len);
+  return n > 1 ? sizeof(float) * (backward ? 3 : 1) * (size_t)B * H * n * dk * dv : 0;
+}
+
+extern "C" int lmufft_decay_attention(const void* q, const void* k, const void* v, int dtype, int64_t ldq, int64_t bsq,
+                                      int64_t ldk, int64_t bsk, int64_t ldv, int64_t bsv, const float* log_decay,
+                                      const int32_t* lengths, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv,
+                                      float scale, void* out, int64_t ldo, int64_t bso, float* state, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  const char* what = "decay attention";
+  if (decay_check(what, dtype, B, T, H, dk, dv)) return 1;
+  if (B == 0 || T == 0) return 0;
+  DecayArgs a{};
+  DecayRole& r = a.role[0];
+  if (decay_tensor(what, "q", q, dtype, ldq, bsq, B, T, (long)H * dk, false, &r.q) ||
+      decay_tensor(what, "k", k, dtype, ldk, bsk, B, T, (long)H * dk, false, &r.k) ||
+      decay_tensor(what, "v", v, dtype, ldv, bsv, B, T, (long)H * dv, false, &r.v) ||
+      decay_tensor(what, "out", out, dtype, ldo, bso, B, T, (long)H * dv, true, &r.out))
+    return 1;
+  if (!log_decay) return set_error("%s: `log_decay` is NULL", what);
+  if (reinterpret_cast<uintptr_t>(state) & 15) return set_error("%s: `state` must be 16-byte aligned", what);
+  a.segments = decay_segments(dtype, B, T, H, dk, dv, &a.seg_len);
+  const size_t need = lmufft_decay_workspace_bytes(dtype, B, T, H, dk, dv, 0);
+  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return set_error("%s: workspace of %zu bytes on a 16-byte boundary needed, %zu given", what, need, workspace_bytes);
+  r.ws = (float*)workspace;
+  a.log_decay = log_decay;
+  a.lengths = lengths;
+  a.state = state;
+  a.scale = scale;
+  a.B = B, a.T = T, a.H = H;
+  return decay_launch_any(dtype, a, 1, dk, dv, (hipStream_t)stream);
+}
+
+extern "C" int lmufft_decay_attention_bwd(const void* q, const void* k, const void* v, const void* dout, int dtype,
+                                          int64_t ldq, int64_t bsq, int64_t ldk, int64_t bsk, int64_t ldv, int64_t bsv,
+                                          int64_t ldd, int64_t bsd, const float* log_decay, const int32_t* lengths,
+                                          int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, float scale, void* dq,
+                                          void* dkey, void* dval, int64_t ld_gq, int64_t bs_gq, int64_t ld_gk,
+                                          int64_t bs_gk, int64_t ld_gv, int64_t bs_gv, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
+  const char* what = "decay attention backward";
+  if (decay_check(what, dtype, B, T, H, dk, dv)) return 1;
+  if (B == 0 || T == 0) return 0;
+  DecayTensor tq, tk, tv, td, gq, gk, gv;
+  if (decay_tensor(what, "q", q, dtype, ldq, bsq, B, T, (long)H * dk, false, &tq) ||
+      decay_tensor(what, "k", k, dtype, ldk, bsk, B, T, (long)H * dk, false, &tk) ||
+      decay_tensor(what, "v", v, dtype, ldv, bsv, B, T, (long)H * dv, false, &tv) ||
+      decay_tensor(what, "dout", dout, dtype, ldd, bsd, B, T, (long)H * dv, false, &td) ||
+      decay_tensor(what, "dq", dq, dtype, ld_gq, bs_gq, B, T, (long)H * dk, true, &gq) ||
+      decay_tensor(what, "dk", dkey, dtype, ld_gk, bs_gk, B, T, (long)H * dk, true, &gk) ||
+      decay_tensor(what, "dv", dval, dtype, ld_gv, bs_gv, B, T, (long)H * dv, true, &gv))
+    return 1;
+  if (!log_decay) return set_error("%s: `log_decay` is NULL", what);
+  DecayArgs a{};
+  a.segments = decay_segments(dtype, B, T, H, dk, dv, &a.seg_len);
+  const size_t need = lmufft_decay_workspace_bytes(dtype, B, T, H, dk, dv, 1);
+  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return set_error("%s: workspace of %zu bytes on a 16-byte boundary needed, %zu given", what, need, workspace_bytes);
+  a.log_decay = log_decay;
+  a.lengths = lengths;
+  a.scale = scale;
+  a.B = B, a.T = T, a.H = H;
+  const size_t part = (size_t)B * H * a.segments * dk * dv;
+  float* const ws = (float*)workspace;
+  // dq = A(do, v, k); dk = A_reversed(v, do, q); dv = A_reversed(k, q, do): one launch when the head widths agree
+  const DecayRole rq = {td, tv, tk, gq, ws, 0}, rk = {tv, td, tq, gk, ws ? ws + part : ws, 1},
+                  rv = {tk, tq, td, gv, ws ? ws + 2 * part : ws, 1};
+  a.role[0] = rq, a.role[1] = rk, a.role[2] = rv;
+  if (dk == dv) return decay_launch_any(dtype, a, 3, dk, dv, (hipStream_t)stream);
+  // the other way round the operator's DK is dv; the segments were chosen for chunks that depend on the type alone
+  if (decay_launch_any(dtype, a, 2, dv, dk, (hipStream_t)stream)) return 1;
+  a.role[0] = rv;
+  return decay_launch_any(dtype, a, 1, dk, dv, (hipStream_t)stream);
+}
+
+extern "C" int lmufft_decay_attention_step(const void* q, const void* k, const void* v, int dtype, int64_t ldq, int64_t ldk,
+                                           int64_t ldv, const float* log_decay, const int32_t* active, int32_t B, int32_t H,
+                                           int32_t dk, int32_t dv, float scale, void* out, int64_t ldo, float* state,
+                                           void* stream) {
+  const char* what = "decay attention step";
+  if (decay_check(what, dtype, B, 1, H, dk, dv)) return 1;
+  if (B == 0) return 0;
+  if (!q || !k || !v || !log_decay || !out || !state) return set_error("%s: NULL pointer", what);
+  if (ldq < 0 || ldk < 0 || ldv < 0 || (B > 1 && ldo < (int64_t)H * dv)) return set_error("%s: bad row stride", what);
+  if (reinterpret_cast<uintptr_t>(state) & 15) return set_error("%s: `state` must be 16-byte aligned", what);
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid((unsigned)(B * H)), block(kDecayStepThreads);
+  {
+    ProfScope ps("k_decay_step", st);
+#define DECAY_STEP(TT, DVV)                                                                                              \
+  hipLaunchKernelGGL((k_decay_step<TT, DVV>), grid, block, 0, st, (const TT*)q, (const TT*)k, (const TT*)v, (long)ldq,    \
+                     (long)ldk, (long)ldv, log_decay, active, H, dk, scale, (TT*)out, (long)ldo, state)
+    if (dtype == LMUFFT_BF16) {
+      if (dv == 32) DECAY_STEP(__bf16, 32);
+      else if (dv == 64) DECAY_STEP(__bf16, 64);
+      else DECAY_STEP(__bf16, 128);
+    } else {
+      if (dv == 32) DECAY_STEP(float, 32);
+      else if (dv == 64) DECAY_STEP(float, 64);
+      else DECAY_STEP(float, 128);
+    }
+#undef DECAY_STEP
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return set_error("launch of k_decay_step failed: %s", hipGetErrorString(e));
+  return 0;
+}

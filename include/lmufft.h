@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define LMUFFT_ABI_VERSION 31
+#define LMUFFT_ABI_VERSION 32
 
 /* element types of the activations (x, h, gh, gx, m) */
 #define LMUFFT_F32 0
@@ -454,6 +454,38 @@ int lmufft_layernorm_param_sum_many(const lmufft_ln_sum_item* items, int32_t cou
  * allocated while such kernels can run.  No counterpart call in the reference.
  * ---------------------------------------------------------------------- */
 int lmufft_dropout_epoch(const uint32_t* epoch_dev);
+
+/* ------------------------------------------------------------------------
+ * Causal linear attention with one decay per head.  No counterpart in the reference, whose attention
+ * (src/models/lmu_encoder.py:48-99) sees whole utterances; this one runs frame by frame as well.  Per head, with
+ * lambda = exp(log_decay[h]) in [0, 1] and a state S [dk][dv]:
+ *   S_t = lambda S_(t-1) + k_t v_t^T,   o_t = scale S_t^T q_t.
+ * q, k [B][T][H * dk], v, out [B][T][H * dv], all f32 or all bf16; ld* / bs* are the element strides of a frame and of an
+ * utterance (rows start on 16-byte boundaries; a column block of a wider tensor is fine, inputs may repeat rows with stride
+ * 0).  lengths [B] (or NULL) is clamped to [0, T]: frames behind it are not read, their outputs and gradients are zeros.
+ * dk, dv in {32, 64, 128}.  Sums and states are held in f32; fixed order, no atomics.
+ *   lmufft_decay_attention: state [B][H][dk][dv] f32 (or NULL: zeros, and nothing is kept) is read as the state before
+ *   the first frame and replaced by the state behind the last frame inside the length.
+ *   lmufft_decay_attention_bwd: gradients of q, k, v for a forward that started from zeros (the decays are constants).
+ *   lmufft_decay_attention_step: one frame of each stream, q, k [B][H * dk], v, out [B][H * dv] with row strides ld*
+ *   (any alignment of the element type); streams whose active[b] (may be NULL) is <= 0 get zeros and keep their state.
+ * Workspace: lmufft_decay_workspace_bytes (0 when there are enough heads to fill the chip without splitting utterances);
+ * its contents do not outlive the call.
+ * ---------------------------------------------------------------------- */
+size_t lmufft_decay_workspace_bytes(int dtype, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int backward);
+int lmufft_decay_attention(const void* q, const void* k, const void* v, int dtype, int64_t ldq, int64_t bsq, int64_t ldk,
+                           int64_t bsk, int64_t ldv, int64_t bsv, const float* log_decay, const int32_t* lengths,
+                           int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, float scale, void* out, int64_t ldo,
+                           int64_t bso, float* state, void* workspace, size_t workspace_bytes, void* stream);
+int lmufft_decay_attention_bwd(const void* q, const void* k, const void* v, const void* dout, int dtype, int64_t ldq,
+                               int64_t bsq, int64_t ldk, int64_t bsk, int64_t ldv, int64_t bsv, int64_t ldd, int64_t bsd,
+                               const float* log_decay, const int32_t* lengths, int32_t B, int32_t T, int32_t H,
+                               int32_t dk, int32_t dv, float scale, void* dq, void* dkey, void* dval, int64_t ld_gq,
+                               int64_t bs_gq, int64_t ld_gk, int64_t bs_gk, int64_t ld_gv, int64_t bs_gv,
+                               void* workspace, size_t workspace_bytes, void* stream);
+int lmufft_decay_attention_step(const void* q, const void* k, const void* v, int dtype, int64_t ldq, int64_t ldk,
+                                int64_t ldv, const float* log_decay, const int32_t* active, int32_t B, int32_t H,
+                                int32_t dk, int32_t dv, float scale, void* out, int64_t ldo, float* state, void* stream);
 
 /* ------------------------------------------------------------------------
  * Weight and bias gradient of a Linear layer under bf16 autocast (training).  Replaces what autograd runs

@@ -20,7 +20,7 @@ CONV_TOEPLITZ = 1
 CONV_FFT = 2
 CONV_SCAN = 3
 NOALLOC_SCRATCH_BYTES = 8 << 20
-ABI_VERSION = 32
+ABI_VERSION = 33
 
 
 class Shape(ctypes.Structure):
@@ -269,6 +269,14 @@ def _load():
         f32, vp, vp, vp] + [i64] * 6 + [vp, sz, vp]
     lib.lmufft_decay_attention_step.restype = ci
     lib.lmufft_decay_attention_step.argtypes = [vp, vp, vp, ci, i64, i64, i64, vp, vp, i32, i32, i32, i32, f32, vp, i64, vp, vp]
+    lib.lmufft_group_norm_workspace_bytes.restype = sz
+    lib.lmufft_group_norm_workspace_bytes.argtypes = [i64, i32, i32, i32, ci]
+    lib.lmufft_group_norm.restype = ci
+    lib.lmufft_group_norm.argtypes = [vp, ci, vp, vp, vp, i64, i32, i32, i32, f32, ci, vp, ci, vp, vp, sz, vp]
+    lib.lmufft_group_norm_bwd.restype = ci
+    lib.lmufft_group_norm_bwd.argtypes = [vp, ci, vp, ci, vp, vp, vp, vp, i64, i32, i32, i32, f32, ci, vp, vp, vp, vp, sz, vp]
+    lib.lmufft_dropout_add.restype = ci
+    lib.lmufft_dropout_add.argtypes = [vp, ci, vp, ci, i64, i32, f32, u32, u32, vp, ci, vp]
     lib.lmufft_linear_wprep_bf16.restype = ci
     lib.lmufft_linear_wprep_bf16.argtypes = [vp, vp, i32, i32, i32, vp, vp, i64, vp, vp]
     lib.lmufft_linear_wprep_many_bf16.restype = ci
@@ -356,6 +364,10 @@ EXPORTS = (
     "lmufft_decay_attention",
     "lmufft_decay_attention_bwd",
     "lmufft_decay_attention_step",
+    "lmufft_group_norm_workspace_bytes",
+    "lmufft_group_norm",
+    "lmufft_group_norm_bwd",
+    "lmufft_dropout_add",
     "lmufft_linear_bf16",
     "lmufft_linear_ln_bf16",
     "lmufft_linear_wprep_bf16",

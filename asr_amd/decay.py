@@ -26,6 +26,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+from ._call import dense, frames_of, on_device, ptr
 
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 SUPPORTED_HEAD_WIDTHS = (32, 64, 128)
@@ -67,16 +68,6 @@ def _check_state(what: str, state, q, B: int, H: int, dk: int, dv: int) -> None:
         raise RuntimeError(f"{what}: `state` is replaced in place and must not require a gradient")
 
 
-def _lengths(what: str, lengths, q, B: int):
-    if lengths is None:
-        return None
-    if lengths.shape != (B,):
-        raise RuntimeError(f"{what}: lengths must have shape ({B},), got {tuple(lengths.shape)}")
-    if lengths.dtype != torch.int32 or lengths.device != q.device or not lengths.is_contiguous():
-        lengths = lengths.to(device=q.device, dtype=torch.int32).contiguous()
-    return lengths
-
-
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """`t` [B, T, C] with rows the kernels can load 16 bytes at a time; a column block of a wider tensor stays in place."""
     per = 16 // t.element_size()
@@ -86,29 +77,6 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-class _on:
-    """The device of a call made current for it (hardly ever needed: a switch costs microseconds a call)."""
-
-    def __init__(self, device):
-        self.device = device
-        self.guard = None
-
-    def __enter__(self):
-        if torch.cuda.current_device() != self.device.index:
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
 def _forward(what, q, k, v, num_heads, dk, dv, log_decay, lengths, state, scale):
     B, T, _ = q.shape
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
@@ -116,11 +84,11 @@ def _forward(what, q, k, v, num_heads, dk, dv, log_decay, lengths, state, scale)
     out = torch.empty((B, T, num_heads * dv), dtype=q.dtype, device=q.device)
     size = _lib.lib.lmufft_decay_workspace_bytes(dt, B, T, num_heads, dk, dv, 0)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    with _on(q.device) as stream:
+    with on_device(q.device) as stream:
         rc = _lib.lib.lmufft_decay_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, q.stride(1), q.stride(0), k.stride(1), k.stride(0), v.stride(1),
-            v.stride(0), log_decay.data_ptr(), _ptr(lengths), B, T, num_heads, dk, dv, scale, out.data_ptr(), num_heads * dv,
-            T * num_heads * dv, _ptr(state), _ptr(ws), size, stream)
+            v.stride(0), log_decay.data_ptr(), ptr(lengths), B, T, num_heads, dk, dv, scale, out.data_ptr(), num_heads * dv,
+            T * num_heads * dv, ptr(state), ptr(ws), size, stream)
     if rc:
         _lib.check(rc, "lmufft_decay_attention")
     return out
@@ -139,7 +107,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_heads
     B = q.shape[0]
     if state is not None:
         _check_state("decay_attention", state, q, B, num_heads, dk, dv)
-    lengths = _lengths("decay_attention", lengths, q, B)
+    lengths = frames_of("decay_attention", "lengths", lengths, q, B)
     return _forward("decay_attention", q.detach(), k.detach(), v.detach(), num_heads, dk, dv, log_decay.detach(), lengths, state,
                     dk ** -0.5 if scale is None else float(scale))
 
@@ -153,14 +121,14 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_
     dk, dv = _check("decay_attention_step", q, k, v, num_heads, log_decay, 2)
     B = q.shape[0]
     _check_state("decay_attention_step", state, q, B, num_heads, dk, dv)
-    active = _lengths("decay_attention_step", active, q, B)
+    active = frames_of("decay_attention_step", "active", active, q, B)
     q, k, v = (t if t.stride(1) == 1 else t.contiguous() for t in (q, k, v))
     log_decay = log_decay.contiguous()
     out = torch.empty((B, num_heads * dv), dtype=q.dtype, device=q.device)
-    with _on(q.device) as stream:
+    with on_device(q.device) as stream:
         rc = _lib.lib.lmufft_decay_attention_step(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPES[q.dtype], q.stride(0), k.stride(0), v.stride(0),
-            log_decay.data_ptr(), _ptr(active), B, num_heads, dk, dv, dk ** -0.5 if scale is None else float(scale),
+            log_decay.data_ptr(), ptr(active), B, num_heads, dk, dv, dk ** -0.5 if scale is None else float(scale),
             out.data_ptr(), num_heads * dv, state.data_ptr(), stream)
     if rc:
         _lib.check(rc, "lmufft_decay_attention_step")
@@ -175,12 +143,12 @@ def _backward(q, k, v, dout, num_heads, dk, dv, log_decay, lengths, scale, dq, d
     dout = _rows(dout)
     size = _lib.lib.lmufft_decay_workspace_bytes(dt, B, T, num_heads, dk, dv, 1)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    with _on(q.device) as stream:
+    with on_device(q.device) as stream:
         rc = _lib.lib.lmufft_decay_attention_bwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), dt, q.stride(1), q.stride(0), k.stride(1), k.stride(0),
-            v.stride(1), v.stride(0), dout.stride(1), dout.stride(0), log_decay.data_ptr(), _ptr(lengths), B, T, num_heads, dk,
+            v.stride(1), v.stride(0), dout.stride(1), dout.stride(0), log_decay.data_ptr(), ptr(lengths), B, T, num_heads, dk,
             dv, scale, dq.data_ptr(), dkey.data_ptr(), dval.data_ptr(), dq.stride(1), dq.stride(0), dkey.stride(1),
-            dkey.stride(0), dval.stride(1), dval.stride(0), _ptr(ws), size, stream)
+            dkey.stride(0), dval.stride(1), dval.stride(0), ptr(ws), size, stream)
     if rc:
         _lib.check(rc, "lmufft_decay_attention_bwd")
 
@@ -226,7 +194,7 @@ def decay_attention_train(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num
                           lengths: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
     """decay_attention with autograd for q, k and v (states start at zero)."""
     dk, dv = _check("decay_attention_train", q, k, v, num_heads, log_decay, 3)
-    lengths = _lengths("decay_attention_train", lengths, q, q.shape[0])
+    lengths = frames_of("decay_attention_train", "lengths", lengths, q, q.shape[0])
     return _DecayTrain.apply(q, k, v, log_decay.contiguous(), lengths, num_heads, dk, dv,
                              dk ** -0.5 if scale is None else float(scale))
 
@@ -239,6 +207,6 @@ def decay_attention_train_packed(qkv: torch.Tensor, num_heads: int, log_decay: t
         raise RuntimeError(f"decay_attention_train_packed: qkv must be [batch, frames, 3 * channels], got {tuple(qkv.shape)}")
     q, k, v = qkv.detach().chunk(3, dim=-1)
     dk, _ = _check("decay_attention_train_packed", q, k, v, num_heads, log_decay, 3)
-    lengths = _lengths("decay_attention_train_packed", lengths, qkv, qkv.shape[0])
+    lengths = frames_of("decay_attention_train_packed", "lengths", lengths, qkv, qkv.shape[0])
     return _DecayTrainPacked.apply(qkv, log_decay.contiguous(), lengths, num_heads, dk,
                                    dk ** -0.5 if scale is None else float(scale))

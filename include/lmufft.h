@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define LMUFFT_ABI_VERSION 32
+#define LMUFFT_ABI_VERSION 33
 
 /* element types of the activations (x, h, gh, gx, m) */
 #define LMUFFT_F32 0
@@ -486,6 +486,36 @@ int lmufft_decay_attention_bwd(const void* q, const void* k, const void* v, cons
 int lmufft_decay_attention_step(const void* q, const void* k, const void* v, int dtype, int64_t ldq, int64_t ldk,
                                 int64_t ldv, const float* log_decay, const int32_t* active, int32_t B, int32_t H,
                                 int32_t dk, int32_t dv, float scale, void* out, int64_t ldo, float* state, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Group norm with an activation, channels last, and its backward.  No counterpart in the reference (its norms are layer
+ * norms, src/models/lmu_encoder.py:97, 274).  x [N][T][C], f32 or bf16, dense; a sample is one utterance of T frames, with
+ * T = 1 one row; y = act((x - mean) / sqrt(var + eps) * gamma + beta) with mean and (biased) variance over the frames
+ * inside the length and the C / G channels of a group.  act: 0 none, 1 ReLU, 2 SiLU.  lengths [N] (NULL: all T frames)
+ * is clamped to [0, T]; frames behind it are not read, their outputs and gradients are zeros.
+ * C at most 1024, gamma, beta f32 [C], tensors start on 16-byte boundaries; statistics and sums in f32, fixed order.
+ *   lmufft_group_norm: out f32 or bf16; stats [N][G][2] f32 (mean, rstd; may be NULL; not written for T = 1 without lengths) is
+ *   what the backward reads.  In place (out == x) is fine with one dtype.
+ *   lmufft_group_norm_bwd: dx (dtype of x), dgamma, dbeta f32 [C] (zeros for an empty x).
+ * ---------------------------------------------------------------------- */
+size_t lmufft_group_norm_workspace_bytes(int64_t N, int32_t T, int32_t C, int32_t G, int backward);
+int lmufft_group_norm(const void* x, int x_dtype, const float* gamma, const float* beta, const int32_t* lengths,
+                      int64_t N, int32_t T, int32_t C, int32_t G, float eps, int act, void* out, int out_dtype,
+                      float* stats, void* workspace, size_t workspace_bytes, void* stream);
+int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy, int dy_dtype, const float* gamma,
+                          const float* beta, const int32_t* lengths, const float* stats, int64_t N, int32_t T,
+                          int32_t C, int32_t G, float eps, int act, void* dx, float* dgamma, float* dbeta,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Residual dropout: out = res + keep x / (1 - p_drop) on rows of C elements (res may be NULL), the keep decisions by
+ * the hash given at lmufft_attention_fwd_train with rows of C columns and the epoch of lmufft_dropout_epoch; no mask is
+ * stored, and the backward is the same call on the gradient of `out` without `res`.  Replaces nn.Dropout where nothing in
+ * front of it can take it along (src/models/lmu_encoder.py:232).  f32 or bf16 each, dense, 16-byte aligned; out may be x or
+ * res of the same dtype.
+ * ---------------------------------------------------------------------- */
+int lmufft_dropout_add(const void* x, int x_dtype, const void* res, int res_dtype, int64_t rows, int32_t C,
+                       float p_drop, uint32_t seed0, uint32_t seed1, void* out, int out_dtype, void* stream);
 
 /* ------------------------------------------------------------------------
  * Weight and bias gradient of a Linear layer under bf16 autocast (training).  Replaces what autograd runs

@@ -1,48 +1,17 @@
-"""What the bindings of single operators share: the device and stream of a call, and the layouts its kernels read."""
+"""The operators bound through torch_binding.cpp (asr_amd/_torch_ops.so): argument checks, outputs, workspaces and autograd
+functions in C++ around the C ABI of the library that asr_amd/_lib.py has loaded."""
 from __future__ import annotations
 
-import torch
+import ctypes
+import os
 
+import torch  # noqa: F401  (its libraries have to be loaded first)
 
-class on_device:
-    """The device of a call made current for it, and its stream there: `with on_device(x.device) as stream`.  (A guard that
-    switches to the device that is current already would cost microseconds a call.)"""
+from . import _lib
 
-    def __init__(self, device):
-        self.device = device
-        self.guard = None
+if not os.path.exists(os.path.join(os.path.dirname(os.path.abspath(__file__)), "_torch_ops.so")):
+    raise ImportError("asr_amd/_torch_ops.so is missing: build it with `make -C asr_amd/csrc` "
+                      "(or `python -c 'import __graft_entry__ as g; g.build()'`). asr_amd has no CPU or eager fallback.")
+from . import _torch_ops as ops  # noqa: E402
 
-    def __enter__(self):
-        if torch.cuda.current_device() != self.device.index:
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
-
-
-def ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def dense(t: torch.Tensor) -> torch.Tensor:
-    """`t` contiguous from a 16-byte boundary on."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def frames_of(what: str, name: str, counts, like: torch.Tensor, batch: int):
-    """`counts` [batch] (frames of each utterance, or which streams are live) as the kernels read it: int32 on the device
-    of `like`."""
-    if counts is None:
-        return None
-    if counts.shape != (batch,):
-        raise RuntimeError(f"{what}: `{name}` must have shape ({batch},), got {tuple(counts.shape)}")
-    if counts.is_floating_point() or counts.is_complex():
-        raise RuntimeError(f"{what}: `{name}` must hold whole numbers, got {counts.dtype}")
-    if counts.dtype != torch.int32 or counts.device != like.device or not counts.is_contiguous():
-        counts = counts.to(device=like.device, dtype=torch.int32).contiguous()
-    return counts
+ops.bind({name: ctypes.cast(getattr(_lib.lib, name), ctypes.c_void_p).value for name in ops.entries if name})

@@ -16,10 +16,9 @@ import ctypes
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._call import dense, on_device
+from ._call import ops
 
 _EPOCHS = {}  # device index -> int32 tensor [1], registered with the library for that device
 
@@ -63,41 +62,7 @@ def check_capturable(device, p_drop: float, seeds_given: bool) -> None:
         dropout_epoch(device)  # raises with the explanation
 
 
-_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _dropout_calls = 0
-
-
-def _run(x, residual, p_drop, seed0, seed1, out_dtype):
-    """residual + dropout(x), both dense; one pass."""
-    out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    C = x.shape[-1]
-    with on_device(x.device) as stream:
-        rc = _lib.lib.lmufft_dropout_add(
-            x.data_ptr(), _DTYPES[x.dtype], None if residual is None else residual.data_ptr(),
-            0 if residual is None else _DTYPES[residual.dtype], x.numel() // C, C, p_drop, seed0, seed1, out.data_ptr(),
-            _DTYPES[out_dtype], stream)
-    if rc:
-        _lib.check(rc, "lmufft_dropout_add")
-    return out
-
-
-class _DropoutAdd(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p_drop, seed0, seed1, out_dtype):
-        ctx.conf = (p_drop, seed0, seed1, x.dtype, None if residual is None else residual.dtype)
-        return _run(dense(x), None if residual is None else dense(residual), p_drop, seed0, seed1, out_dtype)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        p_drop, seed0, seed1, x_dtype, res_dtype = ctx.conf
-        dx = dres = None
-        if ctx.needs_input_grad[0]:
-            d = dy if dy.dtype in _DTYPES else dy.float()
-            dx = _run(dense(d), None, p_drop, seed0, seed1, x_dtype)
-        if ctx.needs_input_grad[1]:
-            dres = dy.to(res_dtype)
-        return dx, dres, None, None, None, None
 
 
 def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, p_drop: float = 0.1, seeds=None,
@@ -110,28 +75,12 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, p_drop
     counter.  Under HIP graph capture the seeds are frozen and the device's epoch counter gives every replay its own mask
     (see above); without that counter such a capture raises."""
     global _dropout_calls
-    for name, t in (("x", x), ("residual", residual)):
-        if t is None:
-            continue
-        if t.dtype not in _DTYPES:
-            raise RuntimeError(f"dropout_add: `{name}` is {t.dtype}; supported dtypes are float32 and bfloat16")
-        if not t.is_cuda:
-            raise RuntimeError(f"dropout_add: `{name}` lives on {t.device}; the kernel runs only on a GPU "
-                               "(there is no CPU fallback)")
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise RuntimeError(f"dropout_add: x must be [..., channels], got {tuple(x.shape)}")
-    if residual is not None and (residual.shape != x.shape or residual.device != x.device):
-        raise RuntimeError(f"dropout_add: residual {tuple(residual.shape)} on {residual.device} does not match x "
-                           f"{tuple(x.shape)} on {x.device}")
     if not 0.0 <= p_drop < 1.0:
         raise ValueError(f"dropout probability has to be in [0, 1), got {p_drop}")
-    if out_dtype is None:
-        out_dtype = x.dtype if residual is None else torch.promote_types(x.dtype, residual.dtype)
-    if out_dtype not in _DTYPES:
-        raise RuntimeError(f"dropout_add: output dtype {out_dtype} is not supported")
-    check_capturable(x.device, p_drop, seeds is not None)
     if seeds is None:
+        if x.is_cuda:
+            check_capturable(x.device, p_drop, False)
         if p_drop > 0:
             _dropout_calls += 1
         seeds = (torch.initial_seed() & 0xFFFFFFFF, 0x44520000 ^ (_dropout_calls & 0xFFFFFFFF))
-    return _DropoutAdd.apply(x, residual, float(p_drop), int(seeds[0]) & 0xFFFFFFFF, int(seeds[1]) & 0xFFFFFFFF, out_dtype)
+    return ops.dropout_add(x, residual, p_drop, int(seeds[0]) & 0xFFFFFFFF, int(seeds[1]) & 0xFFFFFFFF, out_dtype)

@@ -12,15 +12,18 @@
 // the group allows and one partial sum serves the V values.
 //   rows (T = 1, no lengths): a row's C / V threads hold it in registers -- one read, one write -- and sum a group over its threads by
 //     shuffles when they are a power of two, through LDS otherwise.
-//   utterances: the frames of an utterance are split over workgroups.  k_gn_stats leaves (count, mean, centred second
-//     moment) of each split and group, k_gn_apply joins them and normalises.  The backward does the same with the
-//     per-channel sums of dz and dz xhat, from which the group sums and the parameter gradients both follow.
+//   utterances, columns: where an utterance's frames of a few groups fit the LDS, a workgroup reads them once, keeps them,
+//     and writes the result: one launch, one read, one write.
+//   utterances, splits: otherwise the frames are split over workgroups.  k_gn_stats leaves (count, mean, centred second
+//     moment) of each split and group, k_gn_apply joins them and normalises, reading x again.  The backward does the same
+//     with the per-channel sums of dz and dz xhat, from which the group sums and the parameter gradients both follow.
 // Sums are 32-bit, second moments about a value of the data, never as a difference of large sums; the moments of
 // different threads are joined in 64 bits.  Fixed order, no atomics.  HBM-bound.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <initializer_list>
 
 #include "lmufft.h"
 #include "lmufft_internal.h"
@@ -114,10 +117,33 @@ __device__ __forceinline__ float gn_group_sum(float v, int L, int g0, float* red
   return s;
 }
 
-// ---- rows (T = 1).  The workgroup's threads hold blockDim / (C / V) rows side by side.
-template <bool XB, bool OB, int V, bool POW2>
-__global__ void k_gn_rows(GnArgs a) {
-  __shared__ float red[1024];
+// The row slots' sums of dgamma, dbeta, one element of the vectors at a time (red: two floats a thread); slot < 0: no part.
+template <int V>
+__device__ __forceinline__ void gn_channel_sums(const GnVec<V>& dg, const GnVec<V>& db, int TR, int RB, int slot, float* red,
+                                                float* out_g, float* out_b) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    __syncthreads();
+    *reinterpret_cast<float2*>(red + 2 * threadIdx.x) = make_float2(dg.f[e], db.f[e]);
+    __syncthreads();
+    if (slot == 0) {
+      float t0 = 0.f, t1 = 0.f;
+      for (int i = 0; i < RB; ++i) {
+        const float2 p = *reinterpret_cast<const float2*>(red + 2 * (threadIdx.x + i * TR));
+        t0 += p.x;
+        t1 += p.y;
+      }
+      out_g[e] = t0;
+      out_b[e] = t1;
+    }
+  }
+}
+
+// ---- rows (T = 1).  The workgroup's threads hold blockDim / (C / V) rows side by side, R such blocks of rows at once: R
+// loads in flight a thread, and gamma, beta read once for many rows (one row at a time: 13.6 us for 25600 x 384 bf16).
+template <bool XB, bool OB, int V, bool POW2, int R>
+__global__ __launch_bounds__(R > 1 ? 256 : 1024) void k_gn_rows(GnArgs a) {
+  __shared__ float red[POW2 ? 1 : 1024];
   const int TR = a.C / V, RB = blockDim.x / TR, cg = a.C / a.G, L = cg / V;
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V, g0 = threadIdx.x - (threadIdx.x % TR) % L;
   const bool on = slot < RB;
@@ -127,39 +153,44 @@ __global__ void k_gn_rows(GnArgs a) {
     g = gn_load<false, V>(a.gamma, c);
     bt = gn_load<false, V>(a.beta, c);
   }
-  for (long r0 = (long)blockIdx.x * RB; r0 < a.N; r0 += (long)gridDim.x * RB) {
-    const long row = r0 + slot;
-    const bool live = on && row < a.N;
-    GnVec<V> x;
-    float s = 0.f;
+  for (long r0 = (long)blockIdx.x * RB * R; r0 < a.N; r0 += (long)gridDim.x * RB * R) {
+    GnVec<V> x[R];
+    bool live[R];
 #pragma unroll
-    for (int e = 0; e < V; ++e) x.f[e] = 0.f;
-    if (live) {
-      x = gn_load<XB, V>(a.x, row * a.C + c);
+    for (int i = 0; i < R; ++i) {
+      const long row = r0 + i * RB + slot;
+      live[i] = on && row < a.N;
 #pragma unroll
-      for (int e = 0; e < V; ++e) s += x.f[e];
+      for (int e = 0; e < V; ++e) x[i].f[e] = 0.f;
+      if (live[i]) x[i] = gn_load<XB, V>(a.x, row * a.C + c);
     }
-    const float mean = gn_group_sum<POW2>(s, L, g0, red) * inv_n;
-    s = 0.f;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      x.f[e] -= mean;
-      s += x.f[e] * x.f[e];
-    }
-    const float rstd = rsqrtf(gn_group_sum<POW2>(s, L, g0, red) * inv_n + a.eps);
-    if (live) {
+    for (int i = 0; i < R; ++i) {
+      float s = 0.f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) x.f[e] = gn_act(x.f[e] * rstd * g.f[e] + bt.f[e], a.act);
-      gn_store<OB, V>(a.out, row * a.C + c, x);
+      for (int e = 0; e < V; ++e) s += x[i].f[e];
+      const float mean = gn_group_sum<POW2>(s, L, g0, red) * inv_n;
+      s = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        x[i].f[e] -= mean;
+        s += x[i].f[e] * x[i].f[e];
+      }
+      const float rstd = rsqrtf(gn_group_sum<POW2>(s, L, g0, red) * inv_n + a.eps);
+      if (live[i]) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[i].f[e] = gn_act(x[i].f[e] * rstd * g.f[e] + bt.f[e], a.act);
+        gn_store<OB, V>(a.out, (r0 + i * RB + slot) * a.C + c, x[i]);
+      }
     }
   }
 }
 
 // Backward of the rows: mean and rstd are recomputed; a thread sums dgamma, dbeta of its channels over the rows it visits,
 // the workgroup leaves one partial [2][C] (dgamma, dbeta) in part[blockIdx].
-template <bool XB, bool GB, int V, bool POW2>
-__global__ void k_gn_rows_bwd(GnArgs a) {
-  __shared__ float red[1024 * 2];
+template <bool XB, bool GB, int V, bool POW2, int R>
+__global__ __launch_bounds__(R > 1 ? 256 : 1024) void k_gn_rows_bwd(GnArgs a) {
+  __shared__ float red[(R > 1 ? 256 : 1024) * 2];
   const int TR = a.C / V, RB = blockDim.x / TR, cg = a.C / a.G, L = cg / V;
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V, g0 = threadIdx.x - (threadIdx.x % TR) % L;
   const bool on = slot < RB;
@@ -171,65 +202,57 @@ __global__ void k_gn_rows_bwd(GnArgs a) {
     g = gn_load<false, V>(a.gamma, c);
     bt = gn_load<false, V>(a.beta, c);
   }
-  for (long r0 = (long)blockIdx.x * RB; r0 < a.N; r0 += (long)gridDim.x * RB) {
-    const long row = r0 + slot;
-    const bool live = on && row < a.N;
-    GnVec<V> x, dy;
-    float s = 0.f;
+  for (long r0 = (long)blockIdx.x * RB * R; r0 < a.N; r0 += (long)gridDim.x * RB * R) {
+    GnVec<V> x[R], dy[R];
+    bool live[R];
 #pragma unroll
-    for (int e = 0; e < V; ++e) x.f[e] = dy.f[e] = 0.f;
-    if (live) {
-      x = gn_load<XB, V>(a.x, row * a.C + c);
-      dy = gn_load<GB, V>(a.dy, row * a.C + c);
+    for (int i = 0; i < R; ++i) {
+      const long row = r0 + i * RB + slot;
+      live[i] = on && row < a.N;
 #pragma unroll
-      for (int e = 0; e < V; ++e) s += x.f[e];
+      for (int e = 0; e < V; ++e) x[i].f[e] = dy[i].f[e] = 0.f;
+      if (live[i]) {
+        x[i] = gn_load<XB, V>(a.x, row * a.C + c);
+        dy[i] = gn_load<GB, V>(a.dy, row * a.C + c);
+      }
     }
-    const float mean = gn_group_sum<POW2>(s, L, g0, red) * inv_n;
-    s = 0.f;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      x.f[e] -= mean;
-      s += x.f[e] * x.f[e];
-    }
-    const float rstd = rsqrtf(gn_group_sum<POW2>(s, L, g0, red) * inv_n + a.eps);
-    float s1 = 0.f, s2 = 0.f;
-    if (live) {
+    for (int i = 0; i < R; ++i) {
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += x[i].f[e];
+      const float mean = gn_group_sum<POW2>(s, L, g0, red) * inv_n;
+      s = 0.f;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        x.f[e] *= rstd;  // xhat
-        const float dz = dy.f[e] * gn_slope(x.f[e] * g.f[e] + bt.f[e], a.act);
-        db.f[e] += dz;
-        dg.f[e] += dz * x.f[e];
-        dy.f[e] = dz * g.f[e];
-        s1 += dy.f[e];
-        s2 += dy.f[e] * x.f[e];
+        x[i].f[e] -= mean;
+        s += x[i].f[e] * x[i].f[e];
+      }
+      const float rstd = rsqrtf(gn_group_sum<POW2>(s, L, g0, red) * inv_n + a.eps);
+      float s1 = 0.f, s2 = 0.f;
+      if (live[i]) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          x[i].f[e] *= rstd;  // xhat
+          const float dz = dy[i].f[e] * gn_slope(x[i].f[e] * g.f[e] + bt.f[e], a.act);
+          db.f[e] += dz;
+          dg.f[e] += dz * x[i].f[e];
+          dy[i].f[e] = dz * g.f[e];
+          s1 += dy[i].f[e];
+          s2 += dy[i].f[e] * x[i].f[e];
+        }
+      }
+      s1 = gn_group_sum<POW2>(s1, L, g0, red) * inv_n;
+      s2 = gn_group_sum<POW2>(s2, L, g0, red) * inv_n;
+      if (live[i]) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[i].f[e] = (dy[i].f[e] - s1 - x[i].f[e] * s2) * rstd;
+        gn_store<XB, V>(a.out, (r0 + i * RB + slot) * a.C + c, x[i]);
       }
     }
-    s1 = gn_group_sum<POW2>(s1, L, g0, red) * inv_n;
-    s2 = gn_group_sum<POW2>(s2, L, g0, red) * inv_n;
-    if (live) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) x.f[e] = (dy.f[e] - s1 - x.f[e] * s2) * rstd;
-      gn_store<XB, V>(a.out, row * a.C + c, x);
-    }
   }
-  // the row slots' sums, one channel element of the vectors at a time (red holds two floats a thread)
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    __syncthreads();
-    red[2 * threadIdx.x] = dg.f[e];
-    red[2 * threadIdx.x + 1] = db.f[e];
-    __syncthreads();
-    if (on && slot == 0) {
-      float t0 = 0.f, t1 = 0.f;
-      for (int i = 0; i < RB; ++i) {
-        t0 += red[2 * (threadIdx.x + i * TR)];
-        t1 += red[2 * (threadIdx.x + i * TR) + 1];
-      }
-      a.part[(long)blockIdx.x * 2 * a.C + c + e] = t0;
-      a.part[(long)blockIdx.x * 2 * a.C + a.C + c + e] = t1;
-    }
-  }
+  float* const out = a.part + (long)blockIdx.x * 2 * a.C;
+  gn_channel_sums<V>(dg, db, TR, RB, on ? slot : -1, red, out + c, out + a.C + c);
 }
 
 // (count, mean, M2) of a set of values, and of two disjoint sets together.  Joined in 64 bits: a handful of values a
@@ -246,51 +269,99 @@ __device__ __forceinline__ GnMoment gn_join(const GnMoment& p, const GnMoment& q
 
 __device__ __forceinline__ int gn_len(const GnArgs& a, long n) { return a.lengths ? min(max(a.lengths[n], 0), a.T) : a.T; }
 
-// ---- utterances.  Workgroup (split, n): threads of a row own V channels each, the workgroup's rows of threads take the
-// split's frames in turn.
+// The moments of cnt values from the sum and the sum of squares of their distances from a pivot.
+__device__ __forceinline__ GnMoment gn_moment(double cnt, float pivot, float s, float ss) {
+  if (cnt <= 0.) return GnMoment{0., 0., 0.};
+  const double m2 = (double)ss - (double)s * s / cnt;
+  return GnMoment{cnt, pivot + (double)s / cnt, m2 < 0. ? 0. : m2};
+}
+__device__ __forceinline__ float2 gn_mean_rstd(const GnMoment& t, float eps) {
+  return make_float2((float)t.mean, (float)(1. / sqrt((t.n > 0. ? t.m2 / t.n : 0.) + (double)eps)));
+}
+// frames first..last-1 of this thread's channels: zeros
+template <bool OB, int V>
+__device__ __forceinline__ void gn_zero_frames(const GnArgs& a, long base, int first, int last, int slot, int RB) {
+  GnVec<V> z;
+#pragma unroll
+  for (int e = 0; e < V; ++e) z.f[e] = 0.f;
+  for (int t = first + slot; t < last; t += RB) gn_store<OB, V>(a.out, base + (long)t * a.C, z);
+}
+template <int V>
+__device__ __forceinline__ GnVec<V> gn_dx(const GnVec<V>& x, const GnVec<V>& dy, const GnVec<V>& g, const GnVec<V>& bt,
+                                          const float2& ms, const float2& m, int act) {
+  GnVec<V> d;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const float h = (x.f[e] - ms.x) * ms.y;
+    const float dz = dy.f[e] * gn_slope(h * g.f[e] + bt.f[e], act);
+    d.f[e] = (dz * g.f[e] - m.x - h * m.y) * ms.y;
+  }
+  return d;
+}
+
+// ---- utterances.  Threads of a row own V channels each, the workgroup's rows of threads take its frames in turn.
+//
+// Sums of a group: (sum, sum of squares) of x - pivot over the threads of the group, the pivot being one value of the group
+// that all its threads take, so the partials of a workgroup simply add up.  red: one float2 a thread.  The threads
+// tid / lanes, each team of `lanes` (a power of two up to 64) joining one group at a time, call `put(group, sum, squares)`.
+template <class F>
+__device__ __forceinline__ void gn_join_groups(float s, float ss, int TR, int RB, int L, int G, float2* red, F put) {
+  red[threadIdx.x] = make_float2(s, ss);
+  __syncthreads();
+  const int parts = RB * L;
+  int lanes = 1;
+  while (lanes < 64 && lanes * 8 < parts) lanes <<= 1;
+  const int team = threadIdx.x / lanes, lane = threadIdx.x % lanes;
+  for (int g0 = 0; g0 < G; g0 += blockDim.x / lanes) {  // uniform: the shuffles need every lane
+    const int g = g0 + team;
+    float a = 0.f, b = 0.f;
+    if (g < G)
+      for (int i = lane; i < parts; i += lanes) {
+        const float2 p = red[(i / L) * TR + g * L + i % L];
+        a += p.x;
+        b += p.y;
+      }
+    for (int o = lanes >> 1; o > 0; o >>= 1) {
+      a += __shfl_xor(a, o);
+      b += __shfl_xor(b, o);
+    }
+    if (g < G && lane == 0) put(g, a, b);
+  }
+}
+
+// Workgroup (split, n) of the statistics over several workgroups: each split's moments of each group.
 template <bool XB, int V>
-__global__ void k_gn_stats(GnArgs a) {
-  __shared__ GnMoment red[1024];
-  const int TR = a.C / V, RB = blockDim.x / TR, L = a.C / a.G / V;
+__global__ __launch_bounds__(1024) void k_gn_stats(GnArgs a) {
+  __shared__ float2 red[1024];
+  const int TR = a.C / V, RB = blockDim.x / TR, cg = a.C / a.G, L = cg / V;
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V;
   const long n = blockIdx.y;
   const int t0 = blockIdx.x * a.split_len, t1 = min(t0 + a.split_len, gn_len(a, n));
-  const long base = n * a.T * a.C + c;
-  float cnt = 0.f, s = 0.f, ss = 0.f, pivot = 0.f;
-  if (slot < RB) {
+  const long base = n * a.T * a.C;
+  float s = 0.f, ss = 0.f;
+  if (slot < RB && t0 < t1) {
+    const float pivot = gn_load<XB, 1>(a.x, base + (long)t0 * a.C + c / cg * cg).f[0];
+#pragma unroll 4
     for (int t = t0 + slot; t < t1; t += RB) {
-      const GnVec<V> x = gn_load<XB, V>(a.x, base + (long)t * a.C);
-      if (cnt == 0.f) pivot = x.f[0];  // the second moment is taken about a value of the data
+      const GnVec<V> x = gn_load<XB, V>(a.x, base + (long)t * a.C + c);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float d = x.f[e] - pivot;
         s += d;
         ss += d * d;
       }
-      cnt += V;
     }
   }
-  const double m = cnt > 0.f ? (double)s / cnt : 0.;
-  const double m2 = (double)ss - s * m;
-  red[threadIdx.x] = GnMoment{cnt, pivot + m, m2 < 0. ? 0. : m2};
-  __syncthreads();
-  // a wave joins a group: its lanes take the RB * L partials in turn, then meet in a tree
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int g = wave; g < a.G; g += blockDim.x >> 6) {
-    GnMoment t{0., 0., 0.};
-    for (int i = lane; i < RB * L; i += 64) t = gn_join(t, red[(i / L) * TR + g * L + i % L]);
-    for (int o = 32; o > 0; o >>= 1) {
-      const GnMoment u{__shfl_xor(t.n, o), __shfl_xor(t.mean, o), __shfl_xor(t.m2, o)};
-      t = (lane & o) ? gn_join(u, t) : gn_join(t, u);
-    }
-    if (lane == 0) {
-      *(reinterpret_cast<GnMoment*>(a.part) + (n * a.splits + blockIdx.x) * a.G + g) = t;
-    }
-  }
+  GnMoment* const out = reinterpret_cast<GnMoment*>(a.part) + (n * a.splits + blockIdx.x) * a.G;
+  gn_join_groups(s, ss, TR, RB, L, a.G, red, [&](int g, float u, float v) {
+    const double cnt = (double)max(t1 - t0, 0) * cg;
+    const float pivot = cnt > 0. ? gn_load<XB, 1>(a.x, base + (long)t0 * a.C + g * cg).f[0] : 0.f;
+    out[g] = gn_moment(cnt, pivot, u, v);
+  });
 }
 
 template <bool XB, bool OB, int V>
-__global__ void k_gn_apply(GnArgs a) {
+__global__ __launch_bounds__(1024) void k_gn_apply(GnArgs a) {
   __shared__ float2 st[kGnMaxWidth];  // [G]
   const int TR = a.C / V, RB = blockDim.x / TR, cg = a.C / a.G;
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V;
@@ -298,8 +369,7 @@ __global__ void k_gn_apply(GnArgs a) {
   for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
     GnMoment t{0., 0., 0.};
     for (int s = 0; s < a.splits; ++s) t = gn_join(t, *(reinterpret_cast<const GnMoment*>(a.part) + (n * a.splits + s) * a.G + g));
-    const float rstd = (float)(1. / sqrt((t.n > 0. ? t.m2 / t.n : 0.) + (double)a.eps));
-    st[g] = make_float2((float)t.mean, rstd);
+    st[g] = gn_mean_rstd(t, a.eps);
     if (a.stats && blockIdx.x == 0) *reinterpret_cast<float2*>(a.stats + (n * a.G + g) * 2) = st[g];
   }
   __syncthreads();
@@ -308,23 +378,19 @@ __global__ void k_gn_apply(GnArgs a) {
   const float2 ms = st[c / cg];
   const int len = gn_len(a, n), t0 = blockIdx.x * a.split_len, t1 = min(t0 + a.split_len, a.T);
   const long base = n * a.T * a.C + c;
-  for (int t = t0 + slot; t < t1; t += RB) {
-    GnVec<V> y;
-    if (t < len) {
-      const GnVec<V> x = gn_load<XB, V>(a.x, base + (long)t * a.C);
+#pragma unroll 4
+  for (int t = t0 + slot; t < min(t1, len); t += RB) {
+    GnVec<V> y = gn_load<XB, V>(a.x, base + (long)t * a.C);
 #pragma unroll
-      for (int e = 0; e < V; ++e) y.f[e] = gn_act((x.f[e] - ms.x) * ms.y * g.f[e] + bt.f[e], a.act);
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) y.f[e] = 0.f;
-    }
+    for (int e = 0; e < V; ++e) y.f[e] = gn_act((y.f[e] - ms.x) * ms.y * g.f[e] + bt.f[e], a.act);
     gn_store<OB, V>(a.out, base + (long)t * a.C, y);
   }
+  gn_zero_frames<OB, V>(a, base, max(t0, len), t1, slot, RB);
 }
 
 // part[n][split][2][C]: sums over the split's frames of dz xhat and dz
 template <bool XB, bool GB, int V>
-__global__ void k_gn_bwd_sums(GnArgs a) {
+__global__ __launch_bounds__(1024) void k_gn_bwd_sums(GnArgs a) {
   __shared__ float red[1024 * 2];
   const int TR = a.C / V, RB = blockDim.x / TR, cg = a.C / a.G;
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V;
@@ -338,6 +404,7 @@ __global__ void k_gn_bwd_sums(GnArgs a) {
   if (on) {
     const GnVec<V> g = gn_load<false, V>(a.gamma, c), bt = gn_load<false, V>(a.beta, c);
     const float2 ms = *reinterpret_cast<const float2*>(a.stats + (n * a.G + c / cg) * 2);
+#pragma unroll 4
     for (int t = t0 + slot; t < t1; t += RB) {
       const GnVec<V> x = gn_load<XB, V>(a.x, base + (long)t * a.C), dy = gn_load<GB, V>(a.dy, base + (long)t * a.C);
 #pragma unroll
@@ -350,109 +417,267 @@ __global__ void k_gn_bwd_sums(GnArgs a) {
     }
   }
   float* const out = a.part + (n * a.splits + blockIdx.x) * 2 * a.C;
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    __syncthreads();
-    red[2 * threadIdx.x] = dg.f[e];
-    red[2 * threadIdx.x + 1] = db.f[e];
-    __syncthreads();
-    if (on && slot == 0) {
-      float u0 = 0.f, u1 = 0.f;
-      for (int i = 0; i < RB; ++i) {
-        u0 += red[2 * (threadIdx.x + i * TR)];
-        u1 += red[2 * (threadIdx.x + i * TR) + 1];
-      }
-      out[c + e] = u0;
-      out[a.C + c + e] = u1;
-    }
+  gn_channel_sums<V>(dg, db, TR, RB, on ? slot : -1, red, out + c, out + a.C + c);
+}
+
+// A sample's splits joined: its channel sums in the place of its first split's, and its groups' means
+// (sum gamma dz) / n, (sum gamma dz xhat) / n behind all partials.
+__global__ __launch_bounds__(1024) void k_gn_bwd_join(GnArgs a) {
+  __shared__ float sums[2 * kGnMaxWidth];
+  const long n = blockIdx.x;
+  const int cg = a.C / a.G, len = gn_len(a, n);
+  float* const p = a.part + n * a.splits * 2 * a.C;
+  for (int i = threadIdx.x; i < 2 * a.C; i += blockDim.x) {
+    float t = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) t += p[(long)s * 2 * a.C + i];
+    p[i] = t;
+    sums[i] = t * a.gamma[i < a.C ? i : i - a.C];
+  }
+  __syncthreads();
+  float2* const out = reinterpret_cast<float2*>(a.part + a.N * a.splits * 2 * a.C) + n * a.G;
+  const float inv = len > 0 ? 1.f / ((float)len * (float)cg) : 0.f;
+  for (int g = threadIdx.x >> 6; g < a.G; g += blockDim.x >> 6) {
+    float s1 = 0.f, s2 = 0.f;
+    for (int i = g * cg + (threadIdx.x & 63); i < (g + 1) * cg; i += 64) s1 += sums[a.C + i], s2 += sums[i];
+    for (int o = 32; o > 0; o >>= 1) s1 += __shfl_xor(s1, o), s2 += __shfl_xor(s2, o);
+    if ((threadIdx.x & 63) == 0) out[g] = make_float2(s1 * inv, s2 * inv);
   }
 }
 
-// dx of one split of one utterance, from the group sums of all its splits
+// dx of one split of one utterance
 template <bool XB, bool GB, int V>
-__global__ void k_gn_bwd_apply(GnArgs a) {
-  __shared__ float sums[2 * kGnMaxWidth];
-  __shared__ float2 gs[kGnMaxWidth];
+__global__ __launch_bounds__(1024) void k_gn_bwd_apply(GnArgs a) {
   const int TR = a.C / V, RB = blockDim.x / TR, cg = a.C / a.G;
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V;
   const long n = blockIdx.y;
   const int len = gn_len(a, n);
-  for (int i = threadIdx.x; i < 2 * a.C; i += blockDim.x) {
-    float t = 0.f;
-    for (int s = 0; s < a.splits; ++s) t += a.part[(n * a.splits + s) * 2 * a.C + i];
-    sums[i] = t;
-  }
-  __syncthreads();
-  for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
-    float s1 = 0.f, s2 = 0.f;
-    for (int i = g * cg; i < (g + 1) * cg; ++i) {
-      s1 += a.gamma[i] * sums[a.C + i];
-      s2 += a.gamma[i] * sums[i];
-    }
-    const float inv = len > 0 ? 1.f / ((float)len * (float)cg) : 0.f;
-    gs[g] = make_float2(s1 * inv, s2 * inv);
-  }
-  __syncthreads();
   if (slot >= RB) return;
   const GnVec<V> g = gn_load<false, V>(a.gamma, c), bt = gn_load<false, V>(a.beta, c);
   const float2 ms = *reinterpret_cast<const float2*>(a.stats + (n * a.G + c / cg) * 2);
-  const float2 m = gs[c / cg];
+  const float2 m = reinterpret_cast<const float2*>(a.part + a.N * a.splits * 2 * a.C)[n * a.G + c / cg];
   const int t0 = blockIdx.x * a.split_len, t1 = min(t0 + a.split_len, a.T);
   const long base = n * a.T * a.C + c;
-  for (int t = t0 + slot; t < t1; t += RB) {
-    GnVec<V> d;
-    if (t < len) {
+#pragma unroll 4
+  for (int t = t0 + slot; t < min(t1, len); t += RB) {
+    const GnVec<V> x = gn_load<XB, V>(a.x, base + (long)t * a.C), dy = gn_load<GB, V>(a.dy, base + (long)t * a.C);
+    gn_store<XB, V>(a.out, base + (long)t * a.C, gn_dx<V>(x, dy, g, bt, ms, m, a.act));
+  }
+  gn_zero_frames<XB, V>(a, base, max(t0, len), t1, slot, RB);
+}
+
+// ---- utterances whose group columns fit a workgroup's LDS: one read, one write, one launch.  A workgroup owns one
+// utterance's `width` channels (whole groups); its frames are kept in LDS as they were read.
+// Workgroups of one utterance stay on one XCD (its blocks are dispatched to the eight XCDs in turn): neighbouring columns
+// share 128-byte lines.
+__device__ __forceinline__ bool gn_slab(const GnArgs& a, long* n, int* slab) {
+  const int slabs = a.splits;  // (the plan's count of column blocks)
+  const long j = blockIdx.x >> 3;
+  *n = (j / slabs) * 8 + (blockIdx.x & 7);
+  *slab = (int)(j % slabs);
+  return *n < a.N;
+}
+template <bool BF16>
+__device__ __forceinline__ constexpr int gn_size() { return BF16 ? 2 : 4; }
+
+template <bool XB, bool OB, int V>
+__global__ __launch_bounds__(512) void k_gn_column(GnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char gn_lds[];
+  __shared__ float2 red[512];
+  __shared__ float2 st[512];  // [groups of the block]: no more than its threads of a row
+  long n;
+  int slab;
+  if (!gn_slab(a, &n, &slab)) return;
+  const int width = a.split_len, TR = width / V, RB = blockDim.x / TR, cg = a.C / a.G, L = cg / V, groups = width / cg;
+  const int slot = threadIdx.x / TR, col = (threadIdx.x % TR) * V, c = slab * width + col;
+  const bool on = slot < RB;
+  const int len = gn_len(a, n);
+  const long base = n * a.T * a.C + c;
+  float s = 0.f, ss = 0.f;
+  const float pivot = len > 0 && on ? gn_load<XB, 1>(a.x, n * a.T * a.C + c / cg * cg).f[0] : 0.f;
+  if (on) {
+#pragma unroll 8
+    for (int t = slot; t < len; t += RB) {
+      const GnVec<V> x = gn_load<XB, V>(a.x, base + (long)t * a.C);
+      gn_store<XB, V>(gn_lds, (long)t * width + col, x);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = x.f[e] - pivot;
+        s += d;
+        ss += d * d;
+      }
+    }
+  }
+  gn_join_groups(s, ss, TR, RB, L, groups, red, [&](int g, float u, float v) {
+    const double cnt = (double)len * cg;
+    const float p = len > 0 ? gn_load<XB, 1>(gn_lds, g * cg).f[0] : 0.f;  // the first frame's, as above
+    st[g] = gn_mean_rstd(gn_moment(cnt, p, u, v), a.eps);
+    if (a.stats) *reinterpret_cast<float2*>(a.stats + (n * a.G + slab * groups + g) * 2) = st[g];
+  });
+  __syncthreads();
+  if (!on) return;
+  const GnVec<V> g = gn_load<false, V>(a.gamma, c), bt = gn_load<false, V>(a.beta, c);
+  const float2 ms = st[col / cg];
+#pragma unroll 4
+  for (int t = slot; t < len; t += RB) {
+    GnVec<V> y = gn_load<XB, V>(gn_lds, (long)t * width + col);
+#pragma unroll
+    for (int e = 0; e < V; ++e) y.f[e] = gn_act((y.f[e] - ms.x) * ms.y * g.f[e] + bt.f[e], a.act);
+    gn_store<OB, V>(a.out, base + (long)t * a.C, y);
+  }
+  gn_zero_frames<OB, V>(a, base, len, a.T, slot, RB);
+}
+
+// The same for the backward; part[n][2][C] receives the utterance's sums of dz xhat and dz.
+template <bool XB, bool GB, int V>
+__global__ __launch_bounds__(512) void k_gn_column_bwd(GnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char gn_lds[];
+  __shared__ float red[512 * 2];
+  __shared__ float sums[2 * kGnMaxWidth];
+  __shared__ float2 gs[512];
+  long n;
+  int slab;
+  if (!gn_slab(a, &n, &slab)) return;
+  const int width = a.split_len, TR = width / V, RB = blockDim.x / TR, cg = a.C / a.G, groups = width / cg;
+  const int slot = threadIdx.x / TR, col = (threadIdx.x % TR) * V, c = slab * width + col;
+  const bool on = slot < RB;
+  const int len = gn_len(a, n);
+  const long base = n * a.T * a.C + c;
+  unsigned char* const dy_lds = gn_lds + (((long)a.T * width * gn_size<XB>() + 15) & ~15L);
+  GnVec<V> dg, db, g, bt;
+#pragma unroll
+  for (int e = 0; e < V; ++e) dg.f[e] = db.f[e] = g.f[e] = bt.f[e] = 0.f;
+  float2 ms = make_float2(0.f, 0.f);
+  if (on) {
+    g = gn_load<false, V>(a.gamma, c);
+    bt = gn_load<false, V>(a.beta, c);
+    ms = *reinterpret_cast<const float2*>(a.stats + (n * a.G + c / cg) * 2);
+#pragma unroll 4
+    for (int t = slot; t < len; t += RB) {
       const GnVec<V> x = gn_load<XB, V>(a.x, base + (long)t * a.C), dy = gn_load<GB, V>(a.dy, base + (long)t * a.C);
+      gn_store<XB, V>(gn_lds, (long)t * width + col, x);
+      gn_store<GB, V>(dy_lds, (long)t * width + col, dy);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float h = (x.f[e] - ms.x) * ms.y;
         const float dz = dy.f[e] * gn_slope(h * g.f[e] + bt.f[e], a.act);
-        d.f[e] = (dz * g.f[e] - m.x - h * m.y) * ms.y;
+        db.f[e] += dz;
+        dg.f[e] += dz * h;
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) d.f[e] = 0.f;
     }
-    gn_store<XB, V>(a.out, base + (long)t * a.C, d);
   }
+  gn_channel_sums<V>(dg, db, TR, RB, on ? slot : -1, red, sums + col, sums + width + col);
+  __syncthreads();
+  for (int i = threadIdx.x; i < width; i += blockDim.x) {
+    float* const p = a.part + n * 2 * a.C + slab * width + i;
+    p[0] = sums[i];
+    p[a.C] = sums[width + i];
+  }
+  const float inv = len > 0 ? 1.f / ((float)len * (float)cg) : 0.f;
+  for (int k = threadIdx.x; k < groups; k += blockDim.x) {
+    float s1 = 0.f, s2 = 0.f;
+    for (int i = k * cg; i < (k + 1) * cg; ++i) {
+      const float w = a.gamma[slab * width + i];
+      s1 += w * sums[width + i];
+      s2 += w * sums[i];
+    }
+    gs[k] = make_float2(s1 * inv, s2 * inv);
+  }
+  __syncthreads();
+  if (!on) return;
+  const float2 m = gs[col / cg];
+#pragma unroll 4
+  for (int t = slot; t < len; t += RB) {
+    const GnVec<V> x = gn_load<XB, V>(gn_lds, (long)t * width + col), dy = gn_load<GB, V>(dy_lds, (long)t * width + col);
+    gn_store<XB, V>(a.out, base + (long)t * a.C, gn_dx<V>(x, dy, g, bt, ms, m, a.act));
+  }
+  gn_zero_frames<XB, V>(a, base, len, a.T, slot, RB);
 }
 
 // out[i] = sum of the partials, i < C: dgamma, else dbeta; one wave a column, a fixed order
-__global__ __launch_bounds__(256) void k_gn_params(const float* __restrict__ part, long count, int C,
+__global__ __launch_bounds__(256) void k_gn_params(const float* __restrict__ part, long count, long stride, int C,
                                                    float* __restrict__ dgamma, float* __restrict__ dbeta) {
   const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (i >= 2 * C) return;
   float t = 0.f;
-  for (long b = lane; b < count; b += 64) t += part[b * 2 * C + i];
+  for (long b = lane; b < count; b += 64) t += part[b * stride + i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
   if (lane == 0) (i < C ? dgamma[i] : dbeta[i - C]) = t;
 }
 
 // ---- host side
+enum { kGnRows, kGnColumn, kGnSplit };
 struct GnPlan {
-  int V, threads, splits, split_len;
+  int kind, V, threads, splits, split_len;  // kGnColumn: the number of column blocks and their width
   bool pow2;
-  long row_blocks;
+  int rows_at_once;
+  long blocks;       // rows: workgroups
+  size_t lds;        // kGnColumn: bytes of its frames
 };
-static bool gn_plan(int64_t N, int32_t T, int32_t C, int32_t G, bool wide, GnPlan* p) {
+constexpr size_t kGnColumnLds = 120 * 1024;  // (of 160 KB; the kernels' own arrays take up to 20)
+
+// `bytes`: of a frame's channel that kGnColumn keeps (x, or x and dy).
+static bool gn_plan(int64_t N, int32_t T, int32_t C, int32_t G, bool wide, bool rows, bool backward, int bytes, GnPlan* p) {
   const int cg = C / G;
   p->V = wide ? 8 : 4;  // 16 bytes of bf16, or of f32
   while (cg % p->V) p->V /= 2;
-  const int tr = C / p->V, L = cg / p->V;
+  const int L = cg / p->V;
+  const int tr = C / p->V;
   if (tr > 1024) return false;
+  p->pow2 = (L & (L - 1)) == 0 && L <= 64;
   // whole waves that hold whole rows of threads, 256 where a row fits
   p->threads = tr <= 256 ? std::max(64, (256 / tr * tr + 63) / 64 * 64) : (tr + 63) / 64 * 64;
-  p->pow2 = (L & (L - 1)) == 0 && L <= 64;
   const int rb = p->threads / tr;
-  p->row_blocks = (N + rb - 1) / rb;
-  // utterances: about 2048 workgroups in all, each with at least eight frames for a thread
+  if (rows) {
+    p->kind = kGnRows;
+    p->rows_at_once = p->threads <= 256 && N >= 4L * rb * 512 ? 4 : 1;  // (fewer rows: more workgroups instead)
+    const long n = (long)rb * p->rows_at_once;
+    p->blocks = std::min<long>((N + n - 1) / n, backward ? kGnRowBwdBlocks : 4096);
+    return true;
+  }
+  // Column blocks: whole groups, at least 64 bytes of a frame where the groups allow it, the widest block that still gives a
+  // workgroup for every CU.  Worth it when the chip is full, or when a launch is all that counts.
+  const int least = std::max(1, (64 / bytes + cg - 1) / cg);
+  int best = 0;
+  for (int m = 1; m <= G; ++m) {
+    if (G % m) continue;
+    const int w = m * cg;
+    if ((size_t)T * w * bytes > kGnColumnLds || w / p->V > 512) break;
+    if (m > least && N * (G / m) < 512) break;
+    best = m;
+    if (m >= least && w * bytes >= 128) break;
+  }
+  if (best && (N * (G / best) >= 192 || (size_t)T * best * cg * bytes <= 32 * 1024)) {
+    p->kind = kGnColumn;
+    p->splits = G / best;
+    p->split_len = best * cg;
+    const int tc = p->split_len / p->V;
+    p->threads = std::min(512, std::max(64, (std::min<int>(512, tc * std::max(1, (T + 3) / 4)) + 63) / 64 * 64));
+    if (p->threads < tc) p->threads = (tc + 63) / 64 * 64;
+    p->lds = (size_t)T * p->split_len * bytes + 32;
+    return true;
+  }
+  p->kind = kGnSplit;
+  // about 2048 workgroups in all, each with at least eight frames for a thread
   long s = std::max<long>(1, 2048 / std::max<long>(1, N));
   s = std::min<long>(std::min<long>(s, kGnMaxSplits), std::max<long>(1, T / (8L * rb)));
   p->split_len = (int)((T + s - 1) / s);
   p->splits = p->split_len ? (T + p->split_len - 1) / p->split_len : 1;
   return true;
 }
+static size_t gn_workspace(const GnPlan& p, int64_t N, int32_t C, int32_t G, bool backward) {
+  if (p.kind == kGnRows) return backward ? sizeof(float) * 2 * C * (size_t)p.blocks : 0;
+  if (p.kind == kGnColumn) return backward ? sizeof(float) * 2 * C * (size_t)N : 0;
+  return backward ? sizeof(float) * 2 * ((size_t)N * p.splits * C + (size_t)N * G) : sizeof(GnMoment) * (size_t)N * p.splits * G;
+}
+// More dynamic LDS than the default limit has to be asked for, once for a kernel (and device).
+static int gn_allow_lds(const void* kernel, size_t bytes) {
+  if (bytes <= 48 * 1024) return 0;
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return e == hipSuccess ? 0 : set_error("group norm: %zu bytes of LDS refused: %s", bytes, hipGetErrorString(e));
+}
+static dim3 gn_column_grid(const GnPlan& p, int64_t N) { return dim3((unsigned)((N + 7) / 8 * 8 * p.splits)); }
 
 static int gn_check(const char* what, int x_dtype, int other, int64_t N, int32_t T, int32_t C, int32_t G, int act) {
   auto known = [](int d) { return d == LMUFFT_F32 || d == LMUFFT_BF16; };
@@ -485,14 +710,15 @@ using namespace lmufft;
 
 extern "C" size_t lmufft_group_norm_workspace_bytes(int64_t N, int32_t T, int32_t C, int32_t G, int backward) {
   if (N <= 0 || T <= 0 || C <= 0 || G <= 0 || C % G || C > kGnMaxWidth) return 0;
-  size_t most = 0;
-  for (bool wide : {false, true}) {
-    GnPlan p;
-    if (!gn_plan(N, T, C, G, wide, &p)) return 0;
-    // (one frame: rows, or with lengths the utterances' kernels)
-    if (T == 1 && backward) most = std::max(most, sizeof(float) * 2 * C * (size_t)std::min<long>(p.row_blocks, kGnRowBwdBlocks));
-    if (T > 1 || N <= 65535) most = std::max(most, (size_t)N * p.splits * (backward ? sizeof(float) * 2 * C : sizeof(GnMoment) * G));
-  }
+  size_t most = 0;  // over the dtypes, and for one frame over rows and utterances
+  for (bool wide : {false, true})
+    for (int bytes : backward ? std::initializer_list<int>{4, 6, 8} : std::initializer_list<int>{2, 4})
+      for (bool rows : {false, true}) {
+        GnPlan p;
+        if ((rows && T != 1) || (!rows && N > 65535)) continue;
+        if (!gn_plan(N, T, C, G, wide, rows, backward, bytes, &p)) return 0;
+        most = std::max(most, gn_workspace(p, N, C, G, backward));
+      }
   return most;
 }
 
@@ -507,21 +733,34 @@ extern "C" int lmufft_group_norm(const void* x, int x_dtype, const float* gamma,
   if (!rows && N > 65535) return set_error("%s: %lld utterances (at most 65535)", what, (long long)N);
   if (!gn_aligned(x) || !gn_aligned(gamma) || !gn_aligned(beta) || !gn_aligned(out) || (reinterpret_cast<uintptr_t>(stats) & 7))
     return set_error("%s: tensors must start on 16-byte boundaries", what);
-  const size_t need = lmufft_group_norm_workspace_bytes(N, T, C, G, 0);
-  if (need && (!workspace || workspace_bytes < need || !gn_aligned(workspace)))
-    return set_error("%s: workspace of %zu bytes on a 16-byte boundary needed, %zu given", what, need, workspace_bytes);
   GnPlan p;
   const bool xb = x_dtype == LMUFFT_BF16, ob = out_dtype == LMUFFT_BF16;
-  if (!gn_plan(N, T, C, G, xb && ob, &p)) return set_error("%s: %d channels in %d groups", what, C, G);
+  if (!gn_plan(N, T, C, G, xb && ob, rows, false, xb ? 2 : 4, &p)) return set_error("%s: %d channels in %d groups", what, C, G);
+  const size_t need = gn_workspace(p, N, C, G, false);
+  if (need && (!workspace || workspace_bytes < need || !gn_aligned(workspace)))
+    return set_error("%s: workspace of %zu bytes on a 16-byte boundary needed, %zu given", what, need, workspace_bytes);
   GnArgs a{x, nullptr, gamma, beta, lengths, out, stats, (float*)workspace, eps, (long)N, T, C, G, act, p.splits, p.split_len};
   hipStream_t st = (hipStream_t)stream;
-  if (rows) {
+  const dim3 block(p.threads);
+  if (p.kind == kGnRows) {
     ProfScope ps("k_gn_rows", st);
-    const dim3 grid((unsigned)std::min<long>(p.row_blocks, 256 * 16)), block(p.threads);
-    if (p.pow2) GN_BY_2(xb, ob, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_rows<A, B, V, true>), grid, block, 0, st, a)));
-    else GN_BY_2(xb, ob, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_rows<A, B, V, false>), grid, block, 0, st, a)));
+    const dim3 grid((unsigned)p.blocks);
+#define GN_ROWS(P2, RR) GN_BY_2(xb, ob, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_rows<A, B, V, P2, RR>), grid, block, 0, st, a)))
+    if (p.pow2 && p.rows_at_once == 4) GN_ROWS(true, 4);
+    else if (p.pow2) GN_ROWS(true, 1);
+    else if (p.rows_at_once == 4) GN_ROWS(false, 4);
+    else GN_ROWS(false, 1);
+#undef GN_ROWS
+  } else if (p.kind == kGnColumn) {
+    ProfScope ps("k_gn_column", st);
+    int rc = 0;
+    GN_BY_2(xb, ob, GN_BY_V(p.V, {
+              rc = gn_allow_lds(reinterpret_cast<const void*>(&k_gn_column<A, B, V>), p.lds);
+              if (!rc) hipLaunchKernelGGL((k_gn_column<A, B, V>), gn_column_grid(p, N), block, p.lds, st, a);
+            }));
+    if (rc) return rc;
   } else {
-    const dim3 grid(p.splits, (unsigned)N), block(p.threads);
+    const dim3 grid(p.splits, (unsigned)N);
     {
       ProfScope ps("k_gn_stats", st);
       GN_BY_2(xb, false, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_stats<A, V>), grid, block, 0, st, a); (void)B));
@@ -543,44 +782,62 @@ extern "C" int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy,
   if (!dgamma || !dbeta) return set_error("%s: NULL pointer", what);
   hipStream_t st = (hipStream_t)stream;
   if (N == 0 || T == 0) {  // empty sums
-    hipLaunchKernelGGL(k_gn_params, dim3((2 * C + 3) / 4), dim3(256), 0, st, (const float*)nullptr, 0L, C, dgamma, dbeta);
+    hipLaunchKernelGGL(k_gn_params, dim3((2 * C + 3) / 4), dim3(256), 0, st, (const float*)nullptr, 0L, 0L, C, dgamma, dbeta);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : set_error("launch of k_gn_params failed: %s", hipGetErrorString(e));
   }
-  if (!x || !dy || !gamma || !beta || !dx || (!(T == 1 && !lengths) && !stats)) return set_error("%s: NULL pointer", what);
   const bool rows = T == 1 && !lengths;  // every row a sample of its own
+  if (!x || !dy || !gamma || !beta || !dx || (!rows && !stats)) return set_error("%s: NULL pointer", what);
   if (!rows && N > 65535) return set_error("%s: %lld utterances (at most 65535)", what, (long long)N);
   if (!gn_aligned(x) || !gn_aligned(dy) || !gn_aligned(gamma) || !gn_aligned(beta) || !gn_aligned(dx) ||
       (reinterpret_cast<uintptr_t>(stats) & 7))
     return set_error("%s: tensors must start on 16-byte boundaries", what);
-  const size_t need = lmufft_group_norm_workspace_bytes(N, T, C, G, 1);
-  if (need && (!workspace || workspace_bytes < need || !gn_aligned(workspace)))
-    return set_error("%s: workspace of %zu bytes on a 16-byte boundary needed, %zu given", what, need, workspace_bytes);
   GnPlan p;
   const bool xb = x_dtype == LMUFFT_BF16, gb = dy_dtype == LMUFFT_BF16;
-  if (!gn_plan(N, T, C, G, xb && gb, &p)) return set_error("%s: %d channels in %d groups", what, C, G);
+  if (!gn_plan(N, T, C, G, xb && gb, rows, true, (xb ? 2 : 4) + (gb ? 2 : 4), &p))
+    return set_error("%s: %d channels in %d groups", what, C, G);
+  const size_t need = gn_workspace(p, N, C, G, true);
+  if (need && (!workspace || workspace_bytes < need || !gn_aligned(workspace)))
+    return set_error("%s: workspace of %zu bytes on a 16-byte boundary needed, %zu given", what, need, workspace_bytes);
   GnArgs a{x,  dy, gamma, beta, lengths, dx, const_cast<float*>(stats), (float*)workspace, eps, (long)N, T, C, G, act,
            p.splits, p.split_len};
-  long partials;
-  if (rows) {
+  const dim3 block(p.threads);
+  long partials = N, stride = 2 * C;
+  if (p.kind == kGnRows) {
     ProfScope ps("k_gn_rows_bwd", st);
-    partials = std::min<long>(p.row_blocks, kGnRowBwdBlocks);
-    const dim3 grid((unsigned)partials), block(p.threads);
-    if (p.pow2) GN_BY_2(xb, gb, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_rows_bwd<A, B, V, true>), grid, block, 0, st, a)));
-    else GN_BY_2(xb, gb, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_rows_bwd<A, B, V, false>), grid, block, 0, st, a)));
+    partials = p.blocks;
+    const dim3 grid((unsigned)partials);
+#define GN_ROWS(P2, RR) GN_BY_2(xb, gb, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_rows_bwd<A, B, V, P2, RR>), grid, block, 0, st, a)))
+    if (p.pow2 && p.rows_at_once == 4) GN_ROWS(true, 4);
+    else if (p.pow2) GN_ROWS(true, 1);
+    else if (p.rows_at_once == 4) GN_ROWS(false, 4);
+    else GN_ROWS(false, 1);
+#undef GN_ROWS
+  } else if (p.kind == kGnColumn) {
+    ProfScope ps("k_gn_column_bwd", st);
+    int rc = 0;
+    GN_BY_2(xb, gb, GN_BY_V(p.V, {
+              rc = gn_allow_lds(reinterpret_cast<const void*>(&k_gn_column_bwd<A, B, V>), p.lds);
+              if (!rc) hipLaunchKernelGGL((k_gn_column_bwd<A, B, V>), gn_column_grid(p, N), block, p.lds, st, a);
+            }));
+    if (rc) return rc;
   } else {
-    partials = (long)N * p.splits;
-    const dim3 grid(p.splits, (unsigned)N), block(p.threads);
+    stride *= p.splits;
+    const dim3 grid(p.splits, (unsigned)N);
     {
       ProfScope ps("k_gn_bwd_sums", st);
       GN_BY_2(xb, gb, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_bwd_sums<A, B, V>), grid, block, 0, st, a)));
+    }
+    {
+      ProfScope ps("k_gn_bwd_join", st);
+      hipLaunchKernelGGL(k_gn_bwd_join, dim3((unsigned)N), dim3(std::min(1024, (2 * C + 63) / 64 * 64)), 0, st, a);
     }
     ProfScope ps("k_gn_bwd_apply", st);
     GN_BY_2(xb, gb, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_bwd_apply<A, B, V>), grid, block, 0, st, a)));
   }
   {
     ProfScope ps("k_gn_params", st);
-    hipLaunchKernelGGL(k_gn_params, dim3((2 * C + 3) / 4), dim3(256), 0, st, (const float*)a.part, partials, C, dgamma, dbeta);
+    hipLaunchKernelGGL(k_gn_params, dim3((2 * C + 3) / 4), dim3(256), 0, st, (const float*)a.part, partials, stride, C, dgamma, dbeta);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error("launch of the group norm backward failed: %s", hipGetErrorString(e));

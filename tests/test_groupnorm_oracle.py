@@ -71,7 +71,7 @@ def test_c_entry_points_refuse_before_any_launch():
 
     for call, text in ((dict(dt=3), b"dtype"), (dict(od=-1), b"dtype"), (dict(C=97), b"bad shape"), (dict(G=0), b"bad shape"),
                        (dict(N=-1), b"bad shape"), (dict(C=1028), b"at most"), (dict(act=3), b"activation"), (dict(x=None), b"NULL"),
-                       (dict(out=None), b"NULL"), (dict(x=q), b"16-byte"), (dict(), b"workspace"), (dict(ws=p, n=8), b"workspace"),
+                       (dict(out=None), b"NULL"), (dict(x=q), b"16-byte"), (dict(T=5000), b"workspace"), (dict(T=5000, ws=p, n=8), b"workspace"),
                        (dict(N=70000), b"utterances")):
         assert fwd(**call) != 0 and text in lib.lmufft_last_error(), (call, lib.lmufft_last_error())
     assert fwd(N=0) == 0 and fwd(T=0) == 0

@@ -12,8 +12,8 @@
 // the group allows and one partial sum serves the V values.
 //   rows (T = 1, no lengths): a row's C / V threads hold it in registers -- one read, one write -- and sum a group over its threads by
 //     shuffles when they are a power of two, through LDS otherwise.
-//   utterances, columns: where an utterance's frames of a few groups fit the LDS, a workgroup reads them once, keeps them,
-//     and writes the result: one launch, one read, one write.
+//   utterances, columns: where an utterance's frames of a few groups fit a workgroup's registers, it reads them once, keeps
+//     them, and writes the result: one launch, one read, one write.
 //   utterances, splits: otherwise the frames are split over workgroups.  k_gn_stats leaves (count, mean, centred second
 //     moment) of each split and group, k_gn_apply joins them and normalises, reading x again.  The backward does the same
 //     with the per-channel sums of dz and dz xhat, from which the group sums and the parameter gradients both follow.
@@ -36,15 +36,18 @@ constexpr int kGnRowBwdBlocks = 1024;  // workgroups of the rows backward: each 
 
 enum { kGnNone = 0, kGnRelu = 1, kGnSilu = 2 };
 
+// 1 / (1 + exp(-z)) by the reciprocal instruction (off by at most one step of 2^-23 of the value): an exact division made the
+// kernels bound by their arithmetic.
+__device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 __device__ __forceinline__ float gn_act(float z, int act) {
   if (act == kGnRelu) return z > 0.f ? z : (z == z ? 0.f : z);
-  if (act == kGnSilu) return z / (1.f + __expf(-z));
+  if (act == kGnSilu) return z * gn_sigmoid(z);
   return z;
 }
 __device__ __forceinline__ float gn_slope(float z, int act) {
   if (act == kGnRelu) return z > 0.f ? 1.f : 0.f;
   if (act == kGnSilu) {
-    const float s = 1.f / (1.f + __expf(-z));
+    const float s = gn_sigmoid(z);
     return s * (1.f + z * (1.f - s));
   }
   return 1.f;
@@ -88,6 +91,38 @@ __device__ __forceinline__ void gn_store(void* base, long idx, const GnVec<V>& v
   }
 }
 
+// V neighbouring values as they lie in memory
+template <bool BF16, int V>
+struct GnRaw;
+template <int V>
+struct GnRaw<true, V> {
+  typedef __bf16 vec __attribute__((ext_vector_type(V)));
+  vec v;
+  __device__ __forceinline__ void load(const void* base, long idx) {
+    v = *reinterpret_cast<const vec*>(reinterpret_cast<const __bf16*>(base) + idx);
+  }
+  __device__ __forceinline__ GnVec<V> get() const {
+    GnVec<V> o;
+#pragma unroll
+    for (int e = 0; e < V; ++e) o.f[e] = (float)v[e];
+    return o;
+  }
+};
+template <int V>
+struct GnRaw<false, V> {
+  typedef float vec __attribute__((ext_vector_type(V)));
+  vec v;
+  __device__ __forceinline__ void load(const void* base, long idx) {
+    v = *reinterpret_cast<const vec*>(reinterpret_cast<const float*>(base) + idx);
+  }
+  __device__ __forceinline__ GnVec<V> get() const {
+    GnVec<V> o;
+#pragma unroll
+    for (int e = 0; e < V; ++e) o.f[e] = v[e];
+    return o;
+  }
+};
+
 struct GnArgs {
   const void* x;
   const void* dy;
@@ -102,9 +137,11 @@ struct GnArgs {
   int T, C, G, act, splits, split_len;
 };
 
-// sum over the L neighbouring threads of a group (this thread's first one is g0); red: one float a thread
+// sum over the L neighbouring threads of a group (this thread's first one is g0; `groups` in the workgroup).  POW2: by
+// shuffles.  Otherwise through red (one float a thread, one a group behind them): few threads a group are summed by each of
+// them, many by a team of lanes (125 threads a group, 3000 x 1000 in 8 groups: 50 us if each thread sums them all).
 template <bool POW2>
-__device__ __forceinline__ float gn_group_sum(float v, int L, int g0, float* red) {
+__device__ __forceinline__ float gn_group_sum(float v, int L, int g0, int groups, float* red) {
   if (POW2) {
     for (int o = L >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
     return v;
@@ -113,37 +150,59 @@ __device__ __forceinline__ float gn_group_sum(float v, int L, int g0, float* red
   red[threadIdx.x] = v;
   __syncthreads();
   float s = 0.f;
-  for (int i = 0; i < L; ++i) s += red[g0 + i];
-  return s;
+  if (L <= 16) {
+    for (int i = 0; i < L; ++i) s += red[g0 + i];
+    return s;
+  }
+  const int lanes = L <= 128 ? 16 : 64, lane = threadIdx.x & (lanes - 1);
+  for (int t0 = 0; t0 < groups; t0 += blockDim.x / lanes) {  // uniform: the shuffles need every lane
+    const int t = t0 + threadIdx.x / lanes;
+    s = 0.f;
+    if (t < groups)
+      for (int i = lane; i < L; i += lanes) s += red[t * L + i];
+    for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if (t < groups && lane == 0) red[1024 + t] = s;
+  }
+  __syncthreads();
+  return red[1024 + min(g0 / L, groups - 1)];
 }
 
-// The row slots' sums of dgamma, dbeta, one element of the vectors at a time (red: two floats a thread); slot < 0: no part.
-template <int V>
-__device__ __forceinline__ void gn_channel_sums(const GnVec<V>& dg, const GnVec<V>& db, int TR, int RB, int slot, float* red,
-                                                float* out_g, float* out_b) {
+// Sums over the workgroup's row slots of the threads' dgamma, dbeta, four elements of the vectors at a time: through red
+// (eight floats a thread), a column's RB values joined by a team of lanes, `put(which, column, sum)` by its first (which: 0
+// dgamma, 1 dbeta; columns count from the thread row's first).
+template <int V, class F>
+__device__ __forceinline__ void gn_channel_sums(const GnVec<V>& dg, const GnVec<V>& db, int TR, int RB, int slot, float* red, F put) {
+  constexpr int S = V < 4 ? V : 4;
+  const int tr = threadIdx.x % TR, columns = TR * 2 * S;
+  int lanes = 1;
+  while (lanes < 16 && lanes * 4 < RB) lanes <<= 1;
+  const int team = threadIdx.x / lanes, lane = threadIdx.x % lanes;
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
+  for (int e0 = 0; e0 < V; e0 += S) {
     __syncthreads();
-    *reinterpret_cast<float2*>(red + 2 * threadIdx.x) = make_float2(dg.f[e], db.f[e]);
+    if (slot >= 0) {
+      float* const p = red + (slot * TR + tr) * 2 * S;
+#pragma unroll
+      for (int e = 0; e < S; ++e) p[e] = dg.f[e0 + e], p[S + e] = db.f[e0 + e];
+    }
     __syncthreads();
-    if (slot == 0) {
-      float t0 = 0.f, t1 = 0.f;
-      for (int i = 0; i < RB; ++i) {
-        const float2 p = *reinterpret_cast<const float2*>(red + 2 * (threadIdx.x + i * TR));
-        t0 += p.x;
-        t1 += p.y;
-      }
-      out_g[e] = t0;
-      out_b[e] = t1;
+    for (int k0 = 0; k0 < columns; k0 += blockDim.x / lanes) {  // uniform: the shuffles need every lane
+      const int k = k0 + team;
+      float t = 0.f;
+      if (k < columns)
+        for (int i = lane; i < RB; i += lanes) t += red[i * columns + k];
+      for (int o = lanes >> 1; o > 0; o >>= 1) t += __shfl_xor(t, o);
+      if (k < columns && lane == 0) put((k % (2 * S)) / S, k / (2 * S) * V + e0 + k % S, t);
     }
   }
 }
 
-// ---- rows (T = 1).  The workgroup's threads hold blockDim / (C / V) rows side by side, R such blocks of rows at once: R
-// loads in flight a thread, and gamma, beta read once for many rows (one row at a time: 13.6 us for 25600 x 384 bf16).
-template <bool XB, bool OB, int V, bool POW2, int R>
-__global__ __launch_bounds__(R > 1 ? 256 : 1024) void k_gn_rows(GnArgs a) {
-  __shared__ float red[POW2 ? 1 : 1024];
+// ---- rows (T = 1).  The workgroup's threads hold blockDim / (C / V) rows side by side.  One row a thread at a time: with
+// four in flight the registers cost more waves than the loads gain (25600 x 384 bf16: 13.0 against 10.9 us, backward 28.8
+// against 20.4).
+template <bool XB, bool OB, int V, bool POW2>
+__global__ __launch_bounds__(1024) void k_gn_rows(GnArgs a) {
+  __shared__ float red[POW2 ? 1 : 1024 + 1024];
   const int TR = a.C / V, RB = blockDim.x / TR, cg = a.C / a.G, L = cg / V;
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V, g0 = threadIdx.x - (threadIdx.x % TR) % L;
   const bool on = slot < RB;
@@ -153,44 +212,40 @@ __global__ __launch_bounds__(R > 1 ? 256 : 1024) void k_gn_rows(GnArgs a) {
     g = gn_load<false, V>(a.gamma, c);
     bt = gn_load<false, V>(a.beta, c);
   }
-  for (long r0 = (long)blockIdx.x * RB * R; r0 < a.N; r0 += (long)gridDim.x * RB * R) {
-    GnVec<V> x[R];
-    bool live[R];
+  for (long r0 = (long)blockIdx.x * RB; r0 < a.N; r0 += (long)gridDim.x * RB) {
+    const long row = r0 + slot;
+    const bool live = on && row < a.N;
+    GnVec<V> x;
+    float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const long row = r0 + i * RB + slot;
-      live[i] = on && row < a.N;
+    for (int e = 0; e < V; ++e) x.f[e] = 0.f;
+    if (live) {
+      x = gn_load<XB, V>(a.x, row * a.C + c);
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[i].f[e] = 0.f;
-      if (live[i]) x[i] = gn_load<XB, V>(a.x, row * a.C + c);
+      for (int e = 0; e < V; ++e) s += x.f[e];
     }
+    const float mean = gn_group_sum<POW2>(s, L, g0, RB * a.G, red) * inv_n;
+    s = 0.f;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      float s = 0.f;
+    for (int e = 0; e < V; ++e) {
+      x.f[e] -= mean;
+      s += x.f[e] * x.f[e];
+    }
+    const float rstd = rsqrtf(gn_group_sum<POW2>(s, L, g0, RB * a.G, red) * inv_n + a.eps);
+    if (live) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) s += x[i].f[e];
-      const float mean = gn_group_sum<POW2>(s, L, g0, red) * inv_n;
-      s = 0.f;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        x[i].f[e] -= mean;
-        s += x[i].f[e] * x[i].f[e];
-      }
-      const float rstd = rsqrtf(gn_group_sum<POW2>(s, L, g0, red) * inv_n + a.eps);
-      if (live[i]) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[i].f[e] = gn_act(x[i].f[e] * rstd * g.f[e] + bt.f[e], a.act);
-        gn_store<OB, V>(a.out, (r0 + i * RB + slot) * a.C + c, x[i]);
-      }
+      for (int e = 0; e < V; ++e) x.f[e] = gn_act(x.f[e] * rstd * g.f[e] + bt.f[e], a.act);
+      gn_store<OB, V>(a.out, row * a.C + c, x);
     }
   }
 }
 
 // Backward of the rows: mean and rstd are recomputed; a thread sums dgamma, dbeta of its channels over the rows it visits,
 // the workgroup leaves one partial [2][C] (dgamma, dbeta) in part[blockIdx].
-template <bool XB, bool GB, int V, bool POW2, int R>
-__global__ __launch_bounds__(R > 1 ? 256 : 1024) void k_gn_rows_bwd(GnArgs a) {
-  __shared__ float red[(R > 1 ? 256 : 1024) * 2];
+template <bool XB, bool GB, int V, bool POW2>
+__global__ __launch_bounds__(1024) void k_gn_rows_bwd(GnArgs a) {
+  __shared__ float red[POW2 ? 1 : 1024 + 1024];
+  extern __shared__ float gn_sums[];
   const int TR = a.C / V, RB = blockDim.x / TR, cg = a.C / a.G, L = cg / V;
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V, g0 = threadIdx.x - (threadIdx.x % TR) % L;
   const bool on = slot < RB;
@@ -202,57 +257,50 @@ __global__ __launch_bounds__(R > 1 ? 256 : 1024) void k_gn_rows_bwd(GnArgs a) {
     g = gn_load<false, V>(a.gamma, c);
     bt = gn_load<false, V>(a.beta, c);
   }
-  for (long r0 = (long)blockIdx.x * RB * R; r0 < a.N; r0 += (long)gridDim.x * RB * R) {
-    GnVec<V> x[R], dy[R];
-    bool live[R];
+  for (long r0 = (long)blockIdx.x * RB; r0 < a.N; r0 += (long)gridDim.x * RB) {
+    const long row = r0 + slot;
+    const bool live = on && row < a.N;
+    GnVec<V> x, dy;
+    float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const long row = r0 + i * RB + slot;
-      live[i] = on && row < a.N;
+    for (int e = 0; e < V; ++e) x.f[e] = dy.f[e] = 0.f;
+    if (live) {
+      x = gn_load<XB, V>(a.x, row * a.C + c);
+      dy = gn_load<GB, V>(a.dy, row * a.C + c);
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[i].f[e] = dy[i].f[e] = 0.f;
-      if (live[i]) {
-        x[i] = gn_load<XB, V>(a.x, row * a.C + c);
-        dy[i] = gn_load<GB, V>(a.dy, row * a.C + c);
-      }
+      for (int e = 0; e < V; ++e) s += x.f[e];
     }
+    const float mean = gn_group_sum<POW2>(s, L, g0, RB * a.G, red) * inv_n;
+    s = 0.f;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < V; ++e) s += x[i].f[e];
-      const float mean = gn_group_sum<POW2>(s, L, g0, red) * inv_n;
-      s = 0.f;
+    for (int e = 0; e < V; ++e) {
+      x.f[e] -= mean;
+      s += x.f[e] * x.f[e];
+    }
+    const float rstd = rsqrtf(gn_group_sum<POW2>(s, L, g0, RB * a.G, red) * inv_n + a.eps);
+    float s1 = 0.f, s2 = 0.f;
+    if (live) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        x[i].f[e] -= mean;
-        s += x[i].f[e] * x[i].f[e];
+        x.f[e] *= rstd;  // xhat
+        const float dz = dy.f[e] * gn_slope(x.f[e] * g.f[e] + bt.f[e], a.act);
+        db.f[e] += dz;
+        dg.f[e] += dz * x.f[e];
+        dy.f[e] = dz * g.f[e];
+        s1 += dy.f[e];
+        s2 += dy.f[e] * x.f[e];
       }
-      const float rstd = rsqrtf(gn_group_sum<POW2>(s, L, g0, red) * inv_n + a.eps);
-      float s1 = 0.f, s2 = 0.f;
-      if (live[i]) {
+    }
+    s1 = gn_group_sum<POW2>(s1, L, g0, RB * a.G, red) * inv_n;
+    s2 = gn_group_sum<POW2>(s2, L, g0, RB * a.G, red) * inv_n;
+    if (live) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          x[i].f[e] *= rstd;  // xhat
-          const float dz = dy[i].f[e] * gn_slope(x[i].f[e] * g.f[e] + bt.f[e], a.act);
-          db.f[e] += dz;
-          dg.f[e] += dz * x[i].f[e];
-          dy[i].f[e] = dz * g.f[e];
-          s1 += dy[i].f[e];
-          s2 += dy[i].f[e] * x[i].f[e];
-        }
-      }
-      s1 = gn_group_sum<POW2>(s1, L, g0, red) * inv_n;
-      s2 = gn_group_sum<POW2>(s2, L, g0, red) * inv_n;
-      if (live[i]) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[i].f[e] = (dy[i].f[e] - s1 - x[i].f[e] * s2) * rstd;
-        gn_store<XB, V>(a.out, (r0 + i * RB + slot) * a.C + c, x[i]);
-      }
+      for (int e = 0; e < V; ++e) x.f[e] = (dy.f[e] - s1 - x.f[e] * s2) * rstd;
+      gn_store<XB, V>(a.out, row * a.C + c, x);
     }
   }
   float* const out = a.part + (long)blockIdx.x * 2 * a.C;
-  gn_channel_sums<V>(dg, db, TR, RB, on ? slot : -1, red, out + c, out + a.C + c);
+  gn_channel_sums<V>(dg, db, TR, RB, on ? slot : -1, gn_sums, [&](int which, int i, float s) { out[which * a.C + i] = s; });
 }
 
 // (count, mean, M2) of a set of values, and of two disjoint sets together.  Joined in 64 bits: a handful of values a
@@ -391,7 +439,7 @@ __global__ __launch_bounds__(1024) void k_gn_apply(GnArgs a) {
 // part[n][split][2][C]: sums over the split's frames of dz xhat and dz
 template <bool XB, bool GB, int V>
 __global__ __launch_bounds__(1024) void k_gn_bwd_sums(GnArgs a) {
-  __shared__ float red[1024 * 2];
+  extern __shared__ float gn_sums[];
   const int TR = a.C / V, RB = blockDim.x / TR, cg = a.C / a.G;
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V;
   const long n = blockIdx.y;
@@ -417,7 +465,7 @@ __global__ __launch_bounds__(1024) void k_gn_bwd_sums(GnArgs a) {
     }
   }
   float* const out = a.part + (n * a.splits + blockIdx.x) * 2 * a.C;
-  gn_channel_sums<V>(dg, db, TR, RB, on ? slot : -1, red, out + c, out + a.C + c);
+  gn_channel_sums<V>(dg, db, TR, RB, on ? slot : -1, gn_sums, [&](int which, int i, float s) { out[which * a.C + i] = s; });
 }
 
 // A sample's splits joined: its channel sums in the place of its first split's, and its groups' means
@@ -466,144 +514,171 @@ __global__ __launch_bounds__(1024) void k_gn_bwd_apply(GnArgs a) {
   gn_zero_frames<XB, V>(a, base, max(t0, len), t1, slot, RB);
 }
 
-// ---- utterances whose group columns fit a workgroup's LDS: one read, one write, one launch.  A workgroup owns one
-// utterance's `width` channels (whole groups); its frames are kept in LDS as they were read.
-// Workgroups of one utterance stay on one XCD (its blocks are dispatched to the eight XCDs in turn): neighbouring columns
-// share 128-byte lines.
-__device__ __forceinline__ bool gn_slab(const GnArgs& a, long* n, int* slab) {
-  const int slabs = a.splits;  // (the plan's count of column blocks)
+// ---- utterances whose group columns fit a workgroup's registers: one read, one write, one launch.  A workgroup owns one
+// utterance's `width` channels (whole groups); a thread keeps its up to NV frames as they were read, all loads in flight
+// together.  (Kept in LDS instead, 93 KB a workgroup left eight waves a CU: 64 x 400 x 384 bf16 backward 32 us.)
+// Workgroups of one utterance stay on one XCD (blocks are dispatched to the eight XCDs in turn): neighbouring columns share
+// 128-byte lines.
+__device__ __forceinline__ bool gn_column_place(const GnArgs& a, long* n, int* block) {
+  const int blocks = a.splits;  // (the plan's count of column blocks)
   const long j = blockIdx.x >> 3;
-  *n = (j / slabs) * 8 + (blockIdx.x & 7);
-  *slab = (int)(j % slabs);
+  *n = (j / blocks) * 8 + (blockIdx.x & 7);
+  *block = (int)(j % blocks);
   return *n < a.N;
 }
-template <bool BF16>
-__device__ __forceinline__ constexpr int gn_size() { return BF16 ? 2 : 4; }
 
-template <bool XB, bool OB, int V>
-__global__ __launch_bounds__(512) void k_gn_column(GnArgs a) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char gn_lds[];
-  __shared__ float2 red[512];
-  __shared__ float2 st[512];  // [groups of the block]: no more than its threads of a row
+template <bool XB, bool OB, int V, int NV>
+__global__ __launch_bounds__(1024) void k_gn_column(GnArgs a) {
+  __shared__ float2 red[1024];
+  __shared__ float2 st[1024];  // [groups of the block]: no more than its threads of a row
   long n;
-  int slab;
-  if (!gn_slab(a, &n, &slab)) return;
+  int block;
+  if (!gn_column_place(a, &n, &block)) return;
   const int width = a.split_len, TR = width / V, RB = blockDim.x / TR, cg = a.C / a.G, L = cg / V, groups = width / cg;
-  const int slot = threadIdx.x / TR, col = (threadIdx.x % TR) * V, c = slab * width + col;
+  const int slot = threadIdx.x / TR, col = (threadIdx.x % TR) * V, c = block * width + col;
   const bool on = slot < RB;
-  const int len = gn_len(a, n);
-  const long base = n * a.T * a.C + c;
+  const int len = on ? gn_len(a, n) : 0;
+  const long base = n * a.T * a.C + c, first = n * a.T * a.C + (long)block * width;
+  GnRaw<XB, V> x[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int t = slot + i * RB;
+    if (t < len) x[i].load(a.x, base + (long)t * a.C);
+  }
   float s = 0.f, ss = 0.f;
-  const float pivot = len > 0 && on ? gn_load<XB, 1>(a.x, n * a.T * a.C + c / cg * cg).f[0] : 0.f;
-  if (on) {
-#pragma unroll 8
-    for (int t = slot; t < len; t += RB) {
-      const GnVec<V> x = gn_load<XB, V>(a.x, base + (long)t * a.C);
-      gn_store<XB, V>(gn_lds, (long)t * width + col, x);
+  const float pivot = len > 0 ? gn_load<XB, 1>(a.x, first + col / cg * cg).f[0] : 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (slot + i * RB < len) {
+      const GnVec<V> v = x[i].get();
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float d = x.f[e] - pivot;
+        const float d = v.f[e] - pivot;
         s += d;
         ss += d * d;
       }
     }
   }
   gn_join_groups(s, ss, TR, RB, L, groups, red, [&](int g, float u, float v) {
-    const double cnt = (double)len * cg;
-    const float p = len > 0 ? gn_load<XB, 1>(gn_lds, g * cg).f[0] : 0.f;  // the first frame's, as above
-    st[g] = gn_mean_rstd(gn_moment(cnt, p, u, v), a.eps);
-    if (a.stats) *reinterpret_cast<float2*>(a.stats + (n * a.G + slab * groups + g) * 2) = st[g];
+    const int frames = gn_len(a, n);
+    const float p = frames > 0 ? gn_load<XB, 1>(a.x, first + g * cg).f[0] : 0.f;
+    st[g] = gn_mean_rstd(gn_moment((double)frames * cg, p, u, v), a.eps);
+    if (a.stats) *reinterpret_cast<float2*>(a.stats + (n * a.G + block * groups + g) * 2) = st[g];
   });
   __syncthreads();
   if (!on) return;
   const GnVec<V> g = gn_load<false, V>(a.gamma, c), bt = gn_load<false, V>(a.beta, c);
   const float2 ms = st[col / cg];
-#pragma unroll 4
-  for (int t = slot; t < len; t += RB) {
-    GnVec<V> y = gn_load<XB, V>(gn_lds, (long)t * width + col);
 #pragma unroll
-    for (int e = 0; e < V; ++e) y.f[e] = gn_act((y.f[e] - ms.x) * ms.y * g.f[e] + bt.f[e], a.act);
-    gn_store<OB, V>(a.out, base + (long)t * a.C, y);
+  for (int i = 0; i < NV; ++i) {
+    const int t = slot + i * RB;
+    if (t < len) {
+      GnVec<V> y = x[i].get();
+#pragma unroll
+      for (int e = 0; e < V; ++e) y.f[e] = gn_act((y.f[e] - ms.x) * ms.y * g.f[e] + bt.f[e], a.act);
+      gn_store<OB, V>(a.out, base + (long)t * a.C, y);
+    }
   }
   gn_zero_frames<OB, V>(a, base, len, a.T, slot, RB);
 }
 
-// The same for the backward; part[n][2][C] receives the utterance's sums of dz xhat and dz.
-template <bool XB, bool GB, int V>
-__global__ __launch_bounds__(512) void k_gn_column_bwd(GnArgs a) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char gn_lds[];
-  __shared__ float red[512 * 2];
+// The same for the backward; part[n][2][C] receives the utterance's sums of dz xhat and dz.  dz is kept in place of dy.
+template <bool XB, bool GB, int V, int NV>
+__global__ __launch_bounds__(1024) void k_gn_column_bwd(GnArgs a) {
+  extern __shared__ float gn_sums[];
   __shared__ float sums[2 * kGnMaxWidth];
-  __shared__ float2 gs[512];
+  __shared__ float2 gs[1024];
   long n;
-  int slab;
-  if (!gn_slab(a, &n, &slab)) return;
+  int block;
+  if (!gn_column_place(a, &n, &block)) return;
   const int width = a.split_len, TR = width / V, RB = blockDim.x / TR, cg = a.C / a.G, groups = width / cg;
-  const int slot = threadIdx.x / TR, col = (threadIdx.x % TR) * V, c = slab * width + col;
+  const int slot = threadIdx.x / TR, col = (threadIdx.x % TR) * V, c = block * width + col;
   const bool on = slot < RB;
-  const int len = gn_len(a, n);
+  const int frames = gn_len(a, n), len = on ? frames : 0;
   const long base = n * a.T * a.C + c;
-  unsigned char* const dy_lds = gn_lds + (((long)a.T * width * gn_size<XB>() + 15) & ~15L);
-  GnVec<V> dg, db, g, bt;
+  GnRaw<XB, V> x[NV];
+  GnVec<V> dz[NV];
+  {
+    GnRaw<GB, V> dy[NV];
 #pragma unroll
-  for (int e = 0; e < V; ++e) dg.f[e] = db.f[e] = g.f[e] = bt.f[e] = 0.f;
+    for (int i = 0; i < NV; ++i) {
+      const int t = slot + i * RB;
+      if (t < len) {
+        x[i].load(a.x, base + (long)t * a.C);
+        dy[i].load(a.dy, base + (long)t * a.C);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) dz[i] = dy[i].get();
+  }
+  GnVec<V> dg, db, g;
+#pragma unroll
+  for (int e = 0; e < V; ++e) dg.f[e] = db.f[e] = 0.f;
   float2 ms = make_float2(0.f, 0.f);
   if (on) {
     g = gn_load<false, V>(a.gamma, c);
-    bt = gn_load<false, V>(a.beta, c);
+    const GnVec<V> bt = gn_load<false, V>(a.beta, c);
     ms = *reinterpret_cast<const float2*>(a.stats + (n * a.G + c / cg) * 2);
-#pragma unroll 4
-    for (int t = slot; t < len; t += RB) {
-      const GnVec<V> x = gn_load<XB, V>(a.x, base + (long)t * a.C), dy = gn_load<GB, V>(a.dy, base + (long)t * a.C);
-      gn_store<XB, V>(gn_lds, (long)t * width + col, x);
-      gn_store<GB, V>(dy_lds, (long)t * width + col, dy);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float h = (x.f[e] - ms.x) * ms.y;
-        const float dz = dy.f[e] * gn_slope(h * g.f[e] + bt.f[e], a.act);
-        db.f[e] += dz;
-        dg.f[e] += dz * h;
+    for (int i = 0; i < NV; ++i) {
+      if (slot + i * RB < len) {
+        const GnVec<V> xv = x[i].get();
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float h = (xv.f[e] - ms.x) * ms.y;
+          dz[i].f[e] *= gn_slope(h * g.f[e] + bt.f[e], a.act);
+          db.f[e] += dz[i].f[e];
+          dg.f[e] += dz[i].f[e] * h;
+        }
       }
     }
   }
-  gn_channel_sums<V>(dg, db, TR, RB, on ? slot : -1, red, sums + col, sums + width + col);
+  float* const out = a.part + n * 2 * a.C + block * width;
+  gn_channel_sums<V>(dg, db, TR, RB, on ? slot : -1, gn_sums, [&](int which, int i, float s) {
+    out[which * a.C + i] = s;
+    sums[which * width + i] = s * a.gamma[block * width + i];
+  });
   __syncthreads();
-  for (int i = threadIdx.x; i < width; i += blockDim.x) {
-    float* const p = a.part + n * 2 * a.C + slab * width + i;
-    p[0] = sums[i];
-    p[a.C] = sums[width + i];
-  }
-  const float inv = len > 0 ? 1.f / ((float)len * (float)cg) : 0.f;
+  const float inv = frames > 0 ? 1.f / ((float)frames * (float)cg) : 0.f;
   for (int k = threadIdx.x; k < groups; k += blockDim.x) {
     float s1 = 0.f, s2 = 0.f;
-    for (int i = k * cg; i < (k + 1) * cg; ++i) {
-      const float w = a.gamma[slab * width + i];
-      s1 += w * sums[width + i];
-      s2 += w * sums[i];
-    }
+    for (int i = k * cg; i < (k + 1) * cg; ++i) s1 += sums[width + i], s2 += sums[i];
     gs[k] = make_float2(s1 * inv, s2 * inv);
   }
   __syncthreads();
   if (!on) return;
   const float2 m = gs[col / cg];
-#pragma unroll 4
-  for (int t = slot; t < len; t += RB) {
-    const GnVec<V> x = gn_load<XB, V>(gn_lds, (long)t * width + col), dy = gn_load<GB, V>(dy_lds, (long)t * width + col);
-    gn_store<XB, V>(a.out, base + (long)t * a.C, gn_dx<V>(x, dy, g, bt, ms, m, a.act));
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int t = slot + i * RB;
+    if (t < len) {
+      GnVec<V> d = x[i].get();
+#pragma unroll
+      for (int e = 0; e < V; ++e) d.f[e] = (dz[i].f[e] * g.f[e] - m.x - (d.f[e] - ms.x) * ms.y * m.y) * ms.y;
+      gn_store<XB, V>(a.out, base + (long)t * a.C, d);
+    }
   }
   gn_zero_frames<XB, V>(a, base, len, a.T, slot, RB);
 }
 
-// out[i] = sum of the partials, i < C: dgamma, else dbeta; one wave a column, a fixed order
-__global__ __launch_bounds__(256) void k_gn_params(const float* __restrict__ part, long count, long stride, int C,
-                                                   float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (i >= 2 * C) return;
+// out[i] = sum of the partials, i < C: dgamma, else dbeta.  A workgroup takes 64 columns, its sixteen waves the partials in
+// turn; a fixed order.
+__global__ __launch_bounds__(1024) void k_gn_params(const float* __restrict__ part, long count, long stride, int C,
+                                                    float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  __shared__ float red[1024];
+  const int i = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
   float t = 0.f;
-  for (long b = lane; b < count; b += 64) t += part[b * stride + i];
+  if (i < 2 * C) {
+#pragma unroll 8
+    for (long b = wave; b < count; b += 16) t += part[b * stride + i];
+  }
+  red[threadIdx.x] = t;
+  __syncthreads();
+  if (wave == 0 && i < 2 * C) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
-  if (lane == 0) (i < C ? dgamma[i] : dbeta[i - C]) = t;
+    for (int w = 1; w < 16; ++w) t += red[w * 64 + threadIdx.x];
+    (i < C ? dgamma[i] : dbeta[i - C]) = t;
+  }
 }
 
 // ---- host side
@@ -611,14 +686,26 @@ enum { kGnRows, kGnColumn, kGnSplit };
 struct GnPlan {
   int kind, V, threads, splits, split_len;  // kGnColumn: the number of column blocks and their width
   bool pow2;
-  int rows_at_once;
   long blocks;       // rows: workgroups
-  size_t lds;        // kGnColumn: bytes of its frames
+  int frames;        // kGnColumn: frames a thread keeps
 };
-constexpr size_t kGnColumnLds = 120 * 1024;  // (of 160 KB; the kernels' own arrays take up to 20)
 
-// `bytes`: of a frame's channel that kGnColumn keeps (x, or x and dy).
-static bool gn_plan(int64_t N, int32_t T, int32_t C, int32_t G, bool wide, bool rows, bool backward, int bytes, GnPlan* p) {
+// The smallest workgroup whose threads keep the T frames of `width` channels, eight frames each where that is enough, at most
+// 16 or what 64 registers hold (`words`: half registers of a kept value: x as it lies in memory, and dz).  False if none does.
+static bool gn_column_fits(int T, int width, int V, int words, GnPlan* p) {
+  const int tc = width / V, most = std::min(16, 128 / (V * words));
+  for (int least : {8, 16})
+    for (int threads : {256, 512, 1024}) {
+      if (tc > threads) continue;
+      const int rb = threads / tc, frames = (T + rb - 1) / rb;
+      if (frames > std::min(least, most)) continue;
+      p->threads = std::min(threads, (tc * std::min(rb, T) + 63) / 64 * 64);
+      p->frames = frames;
+      return true;
+    }
+  return false;
+}
+static bool gn_plan(int64_t N, int32_t T, int32_t C, int32_t G, bool wide, bool rows, bool backward, int x_bytes, GnPlan* p) {
   const int cg = C / G;
   p->V = wide ? 8 : 4;  // 16 bytes of bf16, or of f32
   while (cg % p->V) p->V /= 2;
@@ -631,31 +718,30 @@ static bool gn_plan(int64_t N, int32_t T, int32_t C, int32_t G, bool wide, bool 
   const int rb = p->threads / tr;
   if (rows) {
     p->kind = kGnRows;
-    p->rows_at_once = p->threads <= 256 && N >= 4L * rb * 512 ? 4 : 1;  // (fewer rows: more workgroups instead)
-    const long n = (long)rb * p->rows_at_once;
-    p->blocks = std::min<long>((N + n - 1) / n, backward ? kGnRowBwdBlocks : 4096);
+    p->blocks = std::min<long>((N + rb - 1) / rb, backward ? kGnRowBwdBlocks : 4096);
     return true;
   }
-  // Column blocks: whole groups, at least 64 bytes of a frame where the groups allow it, the widest block that still gives a
-  // workgroup for every CU.  Worth it when the chip is full, or when a launch is all that counts.
-  const int least = std::max(1, (64 / bytes + cg - 1) / cg);
+  // Column blocks: whole groups, 64 bytes of a frame at least where the groups allow it, up to 128 while the chip stays
+  // full.  Taken when there are workgroups for most CUs, or when the launches are all that counts.
+  const int words = x_bytes / 2 + (backward ? 2 : 0);
+  const int least = std::max(1, (64 / x_bytes + cg - 1) / cg);
+  GnPlan q = *p;
+  q.V = std::min(4, p->V);  // (eight values a vector would not leave the registers room)
   int best = 0;
   for (int m = 1; m <= G; ++m) {
     if (G % m) continue;
     const int w = m * cg;
-    if ((size_t)T * w * bytes > kGnColumnLds || w / p->V > 512) break;
+    if (!gn_column_fits(T, w, q.V, words, &q)) break;
     if (m > least && N * (G / m) < 512) break;
     best = m;
-    if (m >= least && w * bytes >= 128) break;
+    if (m >= least && w * x_bytes >= 128) break;
   }
-  if (best && (N * (G / best) >= 192 || (size_t)T * best * cg * bytes <= 32 * 1024)) {
+  if (best && (N * (G / best) >= 192 || (size_t)T * best * cg <= 16 * 1024)) {
+    p->V = q.V;
+    gn_column_fits(T, best * cg, p->V, words, p);
     p->kind = kGnColumn;
     p->splits = G / best;
     p->split_len = best * cg;
-    const int tc = p->split_len / p->V;
-    p->threads = std::min(512, std::max(64, (std::min<int>(512, tc * std::max(1, (T + 3) / 4)) + 63) / 64 * 64));
-    if (p->threads < tc) p->threads = (tc + 63) / 64 * 64;
-    p->lds = (size_t)T * p->split_len * bytes + 32;
     return true;
   }
   p->kind = kGnSplit;
@@ -671,12 +757,6 @@ static size_t gn_workspace(const GnPlan& p, int64_t N, int32_t C, int32_t G, boo
   if (p.kind == kGnColumn) return backward ? sizeof(float) * 2 * C * (size_t)N : 0;
   return backward ? sizeof(float) * 2 * ((size_t)N * p.splits * C + (size_t)N * G) : sizeof(GnMoment) * (size_t)N * p.splits * G;
 }
-// More dynamic LDS than the default limit has to be asked for, once for a kernel (and device).
-static int gn_allow_lds(const void* kernel, size_t bytes) {
-  if (bytes <= 48 * 1024) return 0;
-  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  return e == hipSuccess ? 0 : set_error("group norm: %zu bytes of LDS refused: %s", bytes, hipGetErrorString(e));
-}
 static dim3 gn_column_grid(const GnPlan& p, int64_t N) { return dim3((unsigned)((N + 7) / 8 * 8 * p.splits)); }
 
 static int gn_check(const char* what, int x_dtype, int other, int64_t N, int32_t T, int32_t C, int32_t G, int act) {
@@ -689,6 +769,12 @@ static int gn_check(const char* what, int x_dtype, int other, int64_t N, int32_t
 }
 static bool gn_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+#define GN_BY_V4(V_, CALL)                           \
+  do {                                               \
+    if (V_ == 4) { constexpr int V = 4; CALL; }      \
+    else if (V_ == 2) { constexpr int V = 2; CALL; } \
+    else { constexpr int V = 1; CALL; }              \
+  } while (0)
 #define GN_BY_V(V_, CALL)                    \
   do {                                       \
     if (V_ == 8) { constexpr int V = 8; CALL; }      \
@@ -712,7 +798,7 @@ extern "C" size_t lmufft_group_norm_workspace_bytes(int64_t N, int32_t T, int32_
   if (N <= 0 || T <= 0 || C <= 0 || G <= 0 || C % G || C > kGnMaxWidth) return 0;
   size_t most = 0;  // over the dtypes, and for one frame over rows and utterances
   for (bool wide : {false, true})
-    for (int bytes : backward ? std::initializer_list<int>{4, 6, 8} : std::initializer_list<int>{2, 4})
+    for (int bytes : {2, 4})
       for (bool rows : {false, true}) {
         GnPlan p;
         if ((rows && T != 1) || (!rows && N > 65535)) continue;
@@ -745,20 +831,12 @@ extern "C" int lmufft_group_norm(const void* x, int x_dtype, const float* gamma,
   if (p.kind == kGnRows) {
     ProfScope ps("k_gn_rows", st);
     const dim3 grid((unsigned)p.blocks);
-#define GN_ROWS(P2, RR) GN_BY_2(xb, ob, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_rows<A, B, V, P2, RR>), grid, block, 0, st, a)))
-    if (p.pow2 && p.rows_at_once == 4) GN_ROWS(true, 4);
-    else if (p.pow2) GN_ROWS(true, 1);
-    else if (p.rows_at_once == 4) GN_ROWS(false, 4);
-    else GN_ROWS(false, 1);
-#undef GN_ROWS
+    if (p.pow2) GN_BY_2(xb, ob, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_rows<A, B, V, true>), grid, block, 0, st, a)));
+    else GN_BY_2(xb, ob, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_rows<A, B, V, false>), grid, block, 0, st, a)));
   } else if (p.kind == kGnColumn) {
     ProfScope ps("k_gn_column", st);
-    int rc = 0;
-    GN_BY_2(xb, ob, GN_BY_V(p.V, {
-              rc = gn_allow_lds(reinterpret_cast<const void*>(&k_gn_column<A, B, V>), p.lds);
-              if (!rc) hipLaunchKernelGGL((k_gn_column<A, B, V>), gn_column_grid(p, N), block, p.lds, st, a);
-            }));
-    if (rc) return rc;
+    if (p.frames <= 8) GN_BY_2(xb, ob, GN_BY_V4(p.V, hipLaunchKernelGGL((k_gn_column<A, B, V, 8>), gn_column_grid(p, N), block, 0, st, a)));
+    else GN_BY_2(xb, ob, GN_BY_V4(p.V, hipLaunchKernelGGL((k_gn_column<A, B, V, 16>), gn_column_grid(p, N), block, 0, st, a)));
   } else {
     const dim3 grid(p.splits, (unsigned)N);
     {
@@ -782,7 +860,7 @@ extern "C" int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy,
   if (!dgamma || !dbeta) return set_error("%s: NULL pointer", what);
   hipStream_t st = (hipStream_t)stream;
   if (N == 0 || T == 0) {  // empty sums
-    hipLaunchKernelGGL(k_gn_params, dim3((2 * C + 3) / 4), dim3(256), 0, st, (const float*)nullptr, 0L, 0L, C, dgamma, dbeta);
+    hipLaunchKernelGGL(k_gn_params, dim3((2 * C + 63) / 64), dim3(1024), 0, st, (const float*)nullptr, 0L, 0L, C, dgamma, dbeta);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : set_error("launch of k_gn_params failed: %s", hipGetErrorString(e));
   }
@@ -794,7 +872,7 @@ extern "C" int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy,
     return set_error("%s: tensors must start on 16-byte boundaries", what);
   GnPlan p;
   const bool xb = x_dtype == LMUFFT_BF16, gb = dy_dtype == LMUFFT_BF16;
-  if (!gn_plan(N, T, C, G, xb && gb, rows, true, (xb ? 2 : 4) + (gb ? 2 : 4), &p))
+  if (!gn_plan(N, T, C, G, xb && gb, rows, true, xb ? 2 : 4, &p))
     return set_error("%s: %d channels in %d groups", what, C, G);
   const size_t need = gn_workspace(p, N, C, G, true);
   if (need && (!workspace || workspace_bytes < need || !gn_aligned(workspace)))
@@ -803,30 +881,23 @@ extern "C" int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy,
            p.splits, p.split_len};
   const dim3 block(p.threads);
   long partials = N, stride = 2 * C;
+  const size_t lds = sizeof(float) * p.threads * 2 * std::min(4, p.V);  // gn_channel_sums: at most 32 KB
   if (p.kind == kGnRows) {
     ProfScope ps("k_gn_rows_bwd", st);
     partials = p.blocks;
     const dim3 grid((unsigned)partials);
-#define GN_ROWS(P2, RR) GN_BY_2(xb, gb, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_rows_bwd<A, B, V, P2, RR>), grid, block, 0, st, a)))
-    if (p.pow2 && p.rows_at_once == 4) GN_ROWS(true, 4);
-    else if (p.pow2) GN_ROWS(true, 1);
-    else if (p.rows_at_once == 4) GN_ROWS(false, 4);
-    else GN_ROWS(false, 1);
-#undef GN_ROWS
+    if (p.pow2) GN_BY_2(xb, gb, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_rows_bwd<A, B, V, true>), grid, block, lds, st, a)));
+    else GN_BY_2(xb, gb, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_rows_bwd<A, B, V, false>), grid, block, lds, st, a)));
   } else if (p.kind == kGnColumn) {
     ProfScope ps("k_gn_column_bwd", st);
-    int rc = 0;
-    GN_BY_2(xb, gb, GN_BY_V(p.V, {
-              rc = gn_allow_lds(reinterpret_cast<const void*>(&k_gn_column_bwd<A, B, V>), p.lds);
-              if (!rc) hipLaunchKernelGGL((k_gn_column_bwd<A, B, V>), gn_column_grid(p, N), block, p.lds, st, a);
-            }));
-    if (rc) return rc;
+    if (p.frames <= 8) GN_BY_2(xb, gb, GN_BY_V4(p.V, hipLaunchKernelGGL((k_gn_column_bwd<A, B, V, 8>), gn_column_grid(p, N), block, lds, st, a)));
+    else GN_BY_2(xb, gb, GN_BY_V4(p.V, hipLaunchKernelGGL((k_gn_column_bwd<A, B, V, 10>), gn_column_grid(p, N), block, lds, st, a)));
   } else {
     stride *= p.splits;
     const dim3 grid(p.splits, (unsigned)N);
     {
       ProfScope ps("k_gn_bwd_sums", st);
-      GN_BY_2(xb, gb, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_bwd_sums<A, B, V>), grid, block, 0, st, a)));
+      GN_BY_2(xb, gb, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_bwd_sums<A, B, V>), grid, block, lds, st, a)));
     }
     {
       ProfScope ps("k_gn_bwd_join", st);
@@ -837,7 +908,7 @@ extern "C" int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy,
   }
   {
     ProfScope ps("k_gn_params", st);
-    hipLaunchKernelGGL(k_gn_params, dim3((2 * C + 3) / 4), dim3(256), 0, st, (const float*)a.part, partials, stride, C, dgamma, dbeta);
+    hipLaunchKernelGGL(k_gn_params, dim3((2 * C + 63) / 64), dim3(1024), 0, st, (const float*)a.part, partials, stride, C, dgamma, dbeta);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error("launch of the group norm backward failed: %s", hipGetErrorString(e));

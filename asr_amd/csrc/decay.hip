@@ -34,7 +34,7 @@ __global__ __launch_bounds__(kDecayStepThreads) void k_decay_step(const T* __res
   const T* const qp = q + (long)b * ldq + (long)h * DK;
   const T* const kp = k + (long)b * ldk + (long)h * DK;
   const T* const vp = v + (long)b * ldv + (long)h * DV + c;
-  const float lam = exp2f(log_decay[h] * 1.4426950408889634f);
+  const float lam = dec_pow(dec_log2(log_decay[h]), 1);
   dec_f4 vv;
 #pragma unroll
   for (int e = 0; e < 4; ++e) vv[e] = (float)vp[e];
@@ -87,6 +87,7 @@ static int decay_tensor(const char* what, const char* name, const void* p, int d
   if ((reinterpret_cast<uintptr_t>(p) & 15) || ld % unit || bs % unit)
     return set_error("%s: rows of `%s` must start on 16-byte boundaries", what, name);
   if (ld < 0 || bs < 0) return set_error("%s: `%s` has a negative stride", what, name);
+  if (ld > (1 << 22)) return set_error("%s: rows of `%s` are %lld elements apart (at most 2^22)", what, name, (long long)ld);
   if (written && ((T > 1 && ld < width) || (B > 1 && bs < (T - 1) * ld + width)))
     return set_error("%s: rows of `%s` overlap", what, name);
   out->p = p;

@@ -11,21 +11,21 @@
 //   dq = A(do, v, k),   dk = A_reversed(v, do, q),   dv = A_reversed(k, q, do),
 // so one kernel serves both directions and a launch takes up to three such roles.
 //
-// A workgroup owns one (utterance, head, segment of frames) and walks the segment's chunks with the state in
-// registers.  Its waves split the DV columns: a wave holds S[all DK][its columns] as MFMA accumulators and computes
-// O^T[its columns][all frames of the chunk].  With transposed products every intermediate stays in registers, because
-// the accumulator layout of a 16 x 16 tile (lane = column, four consecutive rows) is, two tiles side by side, the operand
-// layout of the next product up to a permutation of the contraction index -- and that permutation is baked into how the
-// operands from memory are stored in LDS:
-//   P^T = K Q^T          A = K rows, B = Q rows            (contraction over DK, permuted in 32s)
-//   O^T = S^T Q^T + V^T P^T     A = S^T from S's accumulators, B = Q rows;  A = V^T columns, B = P^T's accumulators
+// A workgroup of four waves owns one (utterance, head, segment of frames) and walks the segment's chunks.  For the outputs
+// a wave owns sixteen frames of the chunk (and, in chunks of 32, half of the columns); the state is held as MFMA accumulators,
+// its tiles split over the waves.  With transposed products a wave's intermediates stay in its registers, because the
+// accumulator layout of a 16 x 16 tile (lane = column, four consecutive rows) is, two tiles side by side, the operand layout
+// of the next product up to a permutation of the contraction index, which the reads of the other operand follow:
+//   P^T = K Q^T          A = K rows, B = Q rows
+//   O^T = S^T Q^T + V^T P^T     A = S^T rows, B = Q rows;  A = V^T columns, B = P^T's accumulators
 //   S  += K^T (w V)      A = K^T columns, B = V^T columns scaled by lambda^(C-1-j)
-// Only q, k, v go through LDS (k both by rows and by columns); the next chunk's rows are fetched into registers while
-// the present one is computed.  Every wave computes all of P^T: sharing it through LDS would cost a barrier per tile.
+// q, k, v go through LDS by rows, as they lie in memory, and the state in the products' type; columns are read from there by
+// the transposing LDS read (bf16) or element by element (f32).  The next chunk's rows are fetched into registers while the
+// present one is computed, and the state is handed over at the barriers that the tiles need anyway.
 //
 // Rounding: products accumulate in 32 bits and the state is held in 32 bits.  bf16 tensors: P and the copy of S that
 // multiplies q are rounded to bf16 once (what a bf16 operand of the matrix cores costs; each is below the rounding of the
-// output); the scaled v that enters the state is split into three bf16 terms, so the state keeps 24 bits.
+// output); the scaled v that enters the state is split into bf16 terms, three where the state is returned (24 bits are kept).
 // f32 tensors: the exact-f32 matrix instruction throughout.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -117,95 +117,111 @@ __device__ __forceinline__ void dec_store4(__bf16* p, const dec_f4& v) {
   *reinterpret_cast<dec_b4*>(p) = o;
 }
 __device__ __forceinline__ void dec_store4(float* p, const dec_f4& v) { *reinterpret_cast<dec_f4*>(p) = v; }
-
-// lambda^n for n >= 0 from log2 lambda (which is -inf for lambda = 0: lambda^0 is 1 all the same)
-__device__ __forceinline__ float dec_pow(float a2, int n) { return n == 0 ? 1.f : exp2f(a2 * (float)n); }
-
-// Position, inside its 32, of contraction index x in a stored operand: the accumulator pair (tiles 2b, 2b + 1) gives lane
-// group g the indices 4g..4g+3 and 16+4g..16+4g+3, which are stored side by side.
-__device__ __forceinline__ constexpr int dec_perm(int x) { return ((x & 15) >> 2) * 8 + (x >> 4) * 4 + (x & 3); }
-
-// A fetched 16-byte piece of a row goes to LDS by rows: quads of columns at their permuted places.
-__device__ __forceinline__ void dec_put_row(__bf16* row, int c0, const dec_u4& v) {
-  const int base = c0 & ~31, x = c0 & 31;
-  *reinterpret_cast<uint2*>(row + base + dec_perm(x)) = make_uint2(v[0], v[1]);
-  *reinterpret_cast<uint2*>(row + base + dec_perm(x + 4)) = make_uint2(v[2], v[3]);
+__device__ __forceinline__ void dec_store8(__bf16* p, const dec_f4& v, const dec_f4& w) {
+  dec_b8 o;
+  dec_pack(o, v, w);
+  *reinterpret_cast<dec_b8*>(p) = o;
 }
-__device__ __forceinline__ void dec_put_row(float* row, int c0, const dec_u4& v) {
-  *reinterpret_cast<dec_u4*>(row + (c0 & ~31) + dec_perm(c0 & 31)) = v;
+__device__ __forceinline__ void dec_store8(float* p, const dec_f4& v, const dec_f4& w) {
+  dec_store4(p, v);
+  dec_store4(p + 4, w);
 }
-// Four rows' pieces (rows j0..j0+3, j0 a multiple of four) go to LDS by columns: tile[column][permuted row].
-template <int PITCH>
-__device__ __forceinline__ void dec_put_cols(__bf16* tile, int c0, int j0, const dec_u4 v[4]) {
-  __bf16* dst = tile + c0 * PITCH + (j0 & ~31) + dec_perm(j0 & 31);
+
+// lambda^n for n >= 0 from log2 lambda, which is held above -2^100 so that lambda = 0 gives lambda^0 = 1 (and 0 behind it)
+__device__ __forceinline__ float dec_log2(float log_decay) {
+  const float a2 = log_decay * 1.4426950408889634f;
+  return a2 < -0x1p100f ? -0x1p100f : a2;
+}
+__device__ __forceinline__ float dec_pow(float a2, int n) { return __builtin_amdgcn_exp2f(a2 * (float)n); }
+__device__ __forceinline__ float dec_uniform(float x) {
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x)));
+}
+
+// Column fragments of a tile that lies in LDS by rows (pitch P): a lane's eight values are one column of the rows 4g..4g+3 and
+// 16+4g..16+4g+3 behind `tile`, as the accumulators of two tiles hold them.  Lane i of sixteen has the column i.
+// dec_cols_spread: it has the column 8 (i / 4) + i % 4 (of 32; the other sixteen lie four columns on): the accumulators of two
+// such tiles hold eight columns side by side.
+template <int P>
+__device__ __forceinline__ void dec_cols_at(dec_b8& f, const __bf16* a) {
+  typedef dec_b4 __attribute__((address_space(3))) * lds4;
+  const dec_b4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)a);
+  const dec_b4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(a + 16 * P));
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {  // columns c0 + 2e and c0 + 2e + 1 share a 32-bit word of each row
-    const uint2 even = make_uint2(__builtin_amdgcn_perm(v[1][e], v[0][e], 0x05040100u),
-                                  __builtin_amdgcn_perm(v[3][e], v[2][e], 0x05040100u));
-    const uint2 odd = make_uint2(__builtin_amdgcn_perm(v[1][e], v[0][e], 0x07060302u),
-                                 __builtin_amdgcn_perm(v[3][e], v[2][e], 0x07060302u));
-    *reinterpret_cast<uint2*>(dst + (2 * e) * PITCH) = even;
-    *reinterpret_cast<uint2*>(dst + (2 * e + 1) * PITCH) = odd;
-  }
+  for (int e = 0; e < 4; ++e) f[e] = lo[e], f[4 + e] = hi[e];
 }
-template <int PITCH>
-__device__ __forceinline__ void dec_put_cols(float* tile, int c0, int j0, const dec_u4 v[4]) {
-  float* dst = tile + c0 * PITCH + (j0 & ~31) + dec_perm(j0 & 31);
+// (the transposing read: of sixteen lanes, lane 4 q + p addresses four columns, piece p, of row q; lane i receives the four
+// rows' values of the i-th column of the four pieces side by side)
+template <int P>
+__device__ __forceinline__ void dec_cols(dec_b8& f, const __bf16* tile, int l16, int g) {
+  dec_cols_at<P>(f, tile + (4 * g + (l16 >> 2)) * P + 4 * (l16 & 3));
+}
+template <int P>
+__device__ __forceinline__ void dec_cols_spread(dec_b8& f, const __bf16* tile, int l16, int g) {
+  dec_cols_at<P>(f, tile + (4 * g + (l16 >> 2)) * P + 8 * (l16 & 3));
+}
+template <int P>
+__device__ __forceinline__ void dec_cols(DecTraits<float>::frag& f, const float* tile, int l16, int g) {
+  const float* a = tile + 4 * g * P + l16;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    dec_u4 t;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) t[r] = v[r][e];
-    *reinterpret_cast<dec_u4*>(dst + e * PITCH) = t;
-  }
+  for (int e = 0; e < 4; ++e) f.a[e] = a[e * P], f.b[e] = a[(16 + e) * P];
+}
+template <int P>
+__device__ __forceinline__ void dec_cols_spread(DecTraits<float>::frag& f, const float* tile, int l16, int g) {
+  dec_cols<P>(f, tile, 8 * (l16 >> 2) + (l16 & 3), g);
 }
 
-// acc += A^T-free product with B = w * v in the state's precision
-__device__ __forceinline__ void dec_split(const dec_b8& v, const float w[8], dec_b8 s[3]) {
+// w v in TERMS bf16 terms: what is left behind the last is below 2^(-9 TERMS) of the value
+template <int TERMS>
+__device__ __forceinline__ void dec_split(const dec_b8& v, const float w[8], dec_b8 s[TERMS]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float x = (float)v[e] * w[e];
-    const __bf16 h = (__bf16)x;
-    const float r = x - (float)h;  // exact
-    const __bf16 m = (__bf16)r;
-    s[0][e] = h;
-    s[1][e] = m;
-    s[2][e] = (__bf16)(r - (float)m);
+    float x = (float)v[e] * w[e];
+#pragma unroll
+    for (int i = 0; i < TERMS; ++i) {
+      s[i][e] = (__bf16)x;
+      x -= (float)s[i][e];  // exact
+    }
   }
 }
 
 // Geometry of the kernels for one (type, DK, DV).
 template <class T, int DK, int DV>
 struct DecGeo {
-  static constexpr int NW = DV >= 64 ? 4 : 2;       // waves; each owns DV / NW columns of S and O
-  static constexpr int MT = DV / NW / 16;           // 16-column tiles of a wave
-  static constexpr int C = sizeof(T) == 2 ? 64 : 32;  // frames per chunk
-  static constexpr int PAD = 16 / sizeof(T);        // rows 16 bytes longer than 64 words: sixteen rows hit different banks
-  static constexpr int PR = DK + PAD;               // pitch of the tiles stored by rows
-  static constexpr int PC = C + PAD;                // pitch of the tiles stored by columns
+  // frames per chunk: 64, or 32 where the tiles would leave room for one workgroup a CU, and for f32, whose products cost more
+  static constexpr int C = sizeof(T) == 2 && DK + DV < 256 ? 64 : 32;
+  static constexpr int THREADS = 256;
+  static constexpr int WQ = C / 16, WD = 4 / WQ;      // waves over the chunk's frames, over the columns of the outputs
+  static constexpr int MO = DV / 16 / WD;             // column tiles of a wave's outputs
+  static constexpr int MS = DV >= 64 ? DV / 64 : 1;   // column tiles of a wave's part of the state
+  static constexpr int KS = DV >= 64 ? 1 : 2;         // waves over the rows of the state
+  static constexpr int KT = DK / 16 / KS;             // row tiles of a wave's part
+  static constexpr int PAD = 16 / sizeof(T);          // rows 16 bytes longer than their data: sixteen rows hit different banks
+  static constexpr int PK = DK + PAD, PV = DV + PAD;  // pitches of the k, q and state tiles, and of the v tile
   static constexpr int VEC = DecTraits<T>::kVec;
-  static constexpr int THREADS = 64 * NW;
-  static constexpr int UK = (C / 4) * (DK / VEC), UV = (C / 4) * (DV / VEC);  // units: four rows x 16 bytes
-  static constexpr int NK = (UK + THREADS - 1) / THREADS, NV = (UV + THREADS - 1) / THREADS;
-  static constexpr size_t kLdsState = sizeof(T) * ((size_t)DK * PC + (size_t)DV * PC);
-  static constexpr size_t kLdsOut = kLdsState + sizeof(T) * 2 * (size_t)C * PR;
+  static constexpr int NK = C * DK / VEC / THREADS, NV = C * DV / VEC / THREADS;  // 16-byte pieces a thread stages
+  static_assert(NK * VEC * THREADS == C * DK && NV * VEC * THREADS == C * DV, "whole pieces for every thread");
+  static constexpr size_t kLdsState = sizeof(T) * (size_t)C * (PK + PV);
+  static constexpr size_t kLdsOut = kLdsState + sizeof(T) * (size_t)(C + DV) * PK;
+  static constexpr int WAVES = kLdsOut <= 52 * 1024 ? 3 : 2;  // a SIMD: as many workgroups as the LDS holds, and no spills
 };
 
 // OUT: the outputs and, in the last segment, the final state.  !OUT: the states at the ends of all segments but the
 // last (which the OUT kernel joins), from zero or, in the first segment, from the initial state.
-template <class T, int DK, int DV, bool OUT>
-__global__ __launch_bounds__(64 * (DV >= 64 ? 4 : 2)) void k_decay(DecayArgs args) {
+// TERMS: bf16 terms of the scaled v that enters the state (see above): three where the state is returned, two where it only
+// serves outputs that are rounded to bf16 themselves.
+template <class T, int DK, int DV, bool OUT, int TERMS>
+__global__ __launch_bounds__(256, (DecGeo<T, DK, DV>::WAVES)) void k_decay(DecayArgs args) {
   typedef DecGeo<T, DK, DV> G;
   typedef typename DecTraits<T>::frag Frag;
-  constexpr int C = G::C, MT = G::MT, KT = DK / 16, KB = DK / 32, JB = C / 32, IT = C / 16, VEC = G::VEC;
+  constexpr int C = G::C, MS = G::MS, KT = G::KT, MO = G::MO, KB = DK / 32, JB = C / 32, VEC = G::VEC, PK = G::PK, PV = G::PV;
   extern __shared__ __attribute__((aligned(16))) unsigned char dec_lds[];
-  T* const kcol = reinterpret_cast<T*>(dec_lds);  // [DK][C]
-  T* const vcol = kcol + DK * G::PC;              // [DV][C]
-  T* const krow = vcol + DV * G::PC;              // [C][DK]
-  T* const qrow = krow + C * G::PR;               // [C][DK]
+  T* const ktile = reinterpret_cast<T*>(dec_lds);  // [C][DK]
+  T* const vtile = ktile + C * PK;                 // [C][DV]
+  T* const qtile = vtile + C * PV;                 // [C][DK]
+  T* const stile = qtile + C * PK;                 // [DV][DK]: S^T
 
   const DecayRole& R = args.role[blockIdx.z];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int bh = blockIdx.x, b = bh / args.H, h = bh - b * args.H, seg = blockIdx.y;
   const int T_ = args.T;
   const int len = args.lengths ? min(max(args.lengths[b], 0), T_) : T_;
@@ -213,7 +229,9 @@ __global__ __launch_bounds__(64 * (DV >= 64 ? 4 : 2)) void k_decay(DecayArgs arg
   const int end = min(s1, len);  // frames s0..end-1 are computed, end..s1-1 (of the padding) get zeros
   const bool first = s0 == 0, single = args.segments == 1;
   const bool rev = R.reverse != 0;
-  const int col0 = wave * (DV / G::NW);  // this wave's first column
+  // this wave's part of the state: rows srow.., columns scol..; and of the outputs: frames 16 it.., column tiles mo0..
+  const int srow = G::KS == 1 ? 0 : (wave >> 1) * KT * 16, scol = G::KS == 1 ? wave * MS * 16 : (wave & 1) * 16;
+  const int it = wave % G::WQ, mo0 = wave / G::WQ * MO;
 
   if (!OUT) {
     // the last segment's copy of the state has a slot of its own: it may be replaced while others still read it
@@ -226,221 +244,241 @@ __global__ __launch_bounds__(64 * (DV >= 64 ? 4 : 2)) void k_decay(DecayArgs arg
     if (s0 + args.seg_len >= len) return;  // nobody needs the state behind this segment
   }
 
-  const T* const qp = (const T*)R.q.p + (long)b * R.q.bs + (long)h * DK;
-  const T* const kp = (const T*)R.k.p + (long)b * R.k.bs + (long)h * DK;
-  const T* const vp = (const T*)R.v.p + (long)b * R.v.bs + (long)h * DV;
-  const float a2 = args.log_decay[h] * 1.4426950408889634f;
-
-  // ---- the state this segment starts from; tile t = rows 16t..16t+15, this lane: column col0 + 16 m + l16, rows 4g..4g+3
-  dec_f4 S[KT][MT];
-#pragma unroll
-  for (int t = 0; t < KT; ++t)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) S[t][m] = dec_f4(0.f);
-  if (first && args.state && s0 <= len) {
-    // (with several segments the copy is read, see above)
-    const float* sp = OUT && !single ? R.ws + ((long)bh * args.segments + args.segments - 1) * (DK * DV)
-                                     : args.state + (long)bh * DK * DV;
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[t][m][r] = sp[(16 * t + 4 * g + r) * DV + col0 + 16 * m + l16];
-  }
-  if (OUT && !first && s0 < len) {
-    // joined from the states at the ends of the earlier segments: sum over s' < seg of lambda^((seg-1-s') seg_len) E_s'
-    float w = 1.f;
-    const float lamL = dec_pow(a2, args.seg_len);
-    for (int s = seg - 1; s >= 0 && w != 0.f; --s, w *= lamL) {
-      const dec_f4* e = reinterpret_cast<const dec_f4*>(R.ws + ((long)bh * args.segments + s) * (DK * DV)) +
-                        wave * (KT * MT * 64) + lane;
-#pragma unroll
-      for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) S[t][m] += w * e[(t * MT + m) * 64];
-    }
-  }
-
-  // ---- powers of the decay
-  float wdiag[4], woff[4], wfar[IT], fq[IT];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int d = l16 - (4 * g + r);  // i - j inside a tile
-    wdiag[r] = d >= 0 ? dec_pow(a2, max(d, 0)) : 0.f;
-    woff[r] = dec_pow(a2, 16 + d);
-  }
-#pragma unroll
-  for (int t = 0; t < IT; ++t) {
-    wfar[t] = t ? dec_pow(a2, 16 * (t - 1)) : 1.f;
-    fq[t] = dec_pow(a2, 16 * t + l16 + 1);
-  }
-  float wv[JB][8];
-
-  // ---- staging
-  dec_u4 kf[G::NK][4], vf[G::NV][4], qf[G::NK][4];
-  auto fetch_rows = [&](const T* p, long ld, int c0, int j0, int t0, dec_u4 out[4]) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int t = t0 + j0 + r;
-      dec_u4 x = dec_u4(0u);
-      if (t < end) x = *reinterpret_cast<const dec_u4*>(p + (long)(rev ? len - 1 - t : t) * ld + c0);
-      out[r] = x;
-    }
+  // ---- staging: thread -> 16-byte pieces (row, columns) of the chunk's tiles.  A chunk's rows lie at a uniform address, which
+  // is that of its lowest row in memory, plus 32-bit offsets that do not change.
+  auto head = [&](const DecayTensor& x, int width) {
+    return reinterpret_cast<const char*>(x.p) + ((long)b * x.bs + (long)h * width) * (long)sizeof(T);
   };
+  const char *const kbase = head(R.k, DK), *const vbase = head(R.v, DV), *const qbase = OUT ? head(R.q, DK) : nullptr;
+  unsigned koff[G::NK], qoff[OUT ? G::NK : 1], voff[G::NV];
+#pragma unroll
+  for (int n = 0; n < G::NK; ++n) {
+    const int u = tid + n * G::THREADS, row = u / (DK / VEC), c = u % (DK / VEC) * VEC, m = rev ? C - 1 - row : row;
+    koff[n] = (unsigned)((m * R.k.ld + c) * (long)sizeof(T));
+    if (OUT) qoff[n] = (unsigned)((m * R.q.ld + c) * (long)sizeof(T));
+  }
+#pragma unroll
+  for (int n = 0; n < G::NV; ++n) {
+    const int u = tid + n * G::THREADS, row = u / (DV / VEC), c = u % (DV / VEC) * VEC, m = rev ? C - 1 - row : row;
+    voff[n] = (unsigned)((m * R.v.ld + c) * (long)sizeof(T));
+  }
+  dec_u4 kf[G::NK], qf[G::NK], vf[G::NV];
   auto fetch = [&](int t0) {
+    const long low = rev ? len - t0 - C : t0;  // (below zero only where the lanes of those rows do not load)
+    const char* const ka = kbase + low * R.k.ld * (long)sizeof(T);
+    const char* const va = vbase + low * R.v.ld * (long)sizeof(T);
+    const char* const qa = OUT ? qbase + low * R.q.ld * (long)sizeof(T) : nullptr;
+    const int n_rows = end - t0;
+    if (n_rows >= C) {
 #pragma unroll
-    for (int n = 0; n < G::NK; ++n) {
-      const int u = tid + n * G::THREADS, c0 = (u % (DK / VEC)) * VEC, j0 = (u / (DK / VEC)) * 4;
-      if (G::UK % G::THREADS != 0 && u >= G::UK) continue;
-      fetch_rows(kp, R.k.ld, c0, j0, t0, kf[n]);
-      if (OUT) fetch_rows(qp, R.q.ld, c0, j0, t0, qf[n]);
-    }
+      for (int n = 0; n < G::NK; ++n) {
+        kf[n] = *reinterpret_cast<const dec_u4*>(ka + koff[n]);
+        if (OUT) qf[n] = *reinterpret_cast<const dec_u4*>(qa + qoff[n]);
+      }
 #pragma unroll
-    for (int n = 0; n < G::NV; ++n) {
-      const int u = tid + n * G::THREADS, c0 = (u % (DV / VEC)) * VEC, j0 = (u / (DV / VEC)) * 4;
-      if (G::UV % G::THREADS != 0 && u >= G::UV) continue;
-      fetch_rows(vp, R.v.ld, c0, j0, t0, vf[n]);
+      for (int n = 0; n < G::NV; ++n) vf[n] = *reinterpret_cast<const dec_u4*>(va + voff[n]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < G::NK; ++n) {
+        const bool in = (tid + n * G::THREADS) / (DK / VEC) < n_rows;
+        kf[n] = dec_u4(0u);
+        if (in) kf[n] = *reinterpret_cast<const dec_u4*>(ka + koff[n]);
+        if (OUT) {
+          qf[n] = dec_u4(0u);
+          if (in) qf[n] = *reinterpret_cast<const dec_u4*>(qa + qoff[n]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < G::NV; ++n) {
+        vf[n] = dec_u4(0u);
+        if ((tid + n * G::THREADS) / (DV / VEC) < n_rows) vf[n] = *reinterpret_cast<const dec_u4*>(va + voff[n]);
+      }
     }
   };
   auto stage = [&]() {
 #pragma unroll
     for (int n = 0; n < G::NK; ++n) {
-      const int u = tid + n * G::THREADS, c0 = (u % (DK / VEC)) * VEC, j0 = (u / (DK / VEC)) * 4;
-      if (G::UK % G::THREADS != 0 && u >= G::UK) continue;
-      dec_put_cols<G::PC>(kcol, c0, j0, kf[n]);
-      if (OUT) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          dec_put_row(krow + (j0 + r) * G::PR, c0, kf[n][r]);
-          dec_put_row(qrow + (j0 + r) * G::PR, c0, qf[n][r]);
-        }
-      }
+      const int u = tid + n * G::THREADS, at = u / (DK / VEC) * PK + u % (DK / VEC) * VEC;
+      *reinterpret_cast<dec_u4*>(ktile + at) = kf[n];
+      if (OUT) *reinterpret_cast<dec_u4*>(qtile + at) = qf[n];
     }
 #pragma unroll
     for (int n = 0; n < G::NV; ++n) {
-      const int u = tid + n * G::THREADS, c0 = (u % (DV / VEC)) * VEC, j0 = (u / (DV / VEC)) * 4;
-      if (G::UV % G::THREADS != 0 && u >= G::UV) continue;
-      dec_put_cols<G::PC>(vcol, c0, j0, vf[n]);
+      const int u = tid + n * G::THREADS;
+      *reinterpret_cast<dec_u4*>(vtile + u / (DV / VEC) * PV + u % (DV / VEC) * VEC) = vf[n];
     }
   };
-
-  T* const op = (T*)R.out.p + (long)b * R.out.bs + (long)h * DV + col0;
   if (s0 < end) fetch(s0);
+
+  // ---- powers of the decay: lambda^(i-j) is, tile by tile, the one of the places inside the tiles times a uniform one
+  const float a2 = dec_log2(args.log_decay[h]);
+  auto upow = [&](int n) { return dec_uniform(dec_pow(a2, n)); };
+  float wdiag[4], woff[4], wend[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int d = l16 - (4 * g + r);
+    wdiag[r] = dec_pow(a2, max(d, 0));
+    woff[r] = dec_pow(a2, 16 + d);
+    wend[r] = dec_pow(a2, 15 - (4 * g + r));
+  }
+  const float fq = dec_pow(a2, 16 * it + l16 + 1);
+
+  // ---- the state this segment starts from: tile (t, m), this lane: column scol + 16 m + l16, rows srow + 16 t + 4 g + r
+  dec_f4 S[KT][MS];
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int m = 0; m < MS; ++m) S[t][m] = dec_f4(0.f);
+  const int splace = (srow + 4 * g) * DV + scol + l16;
+  const int wplace = wave * (KT * MS * 64) + lane;  // in the workspace the accumulators lie as they are
+  if (first && args.state) {
+    // (with several segments the copy is read, see above)
+    const float* sp = (OUT && !single ? R.ws + ((long)bh * args.segments + args.segments - 1) * (DK * DV)
+                                      : args.state + (long)bh * DK * DV) + splace;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int m = 0; m < MS; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[t][m][r] = sp[(16 * t + r) * DV + 16 * m];
+  }
+  if (OUT && !first && s0 < len) {
+    // joined from the states at the ends of the earlier segments: sum over s' < seg of lambda^((seg-1-s') seg_len) E_s'
+    float w = 1.f;
+    const float lamL = upow(args.seg_len);
+    for (int s = seg - 1; s >= 0 && w != 0.f; --s, w *= lamL) {
+      const dec_f4* e = reinterpret_cast<const dec_f4*>(R.ws + ((long)bh * args.segments + s) * (DK * DV)) + wplace;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int m = 0; m < MS; ++m) S[t][m] += w * e[(t * MS + m) * 64];
+    }
+  }
+
+  T* const op = (T*)R.out.p + (long)b * R.out.bs + (long)h * DV + 8 * g;
   for (int t0 = s0; t0 < end; t0 += C) {
     const int n = min(C, end - t0);  // frames of this chunk
     __syncthreads();                 // everybody has finished with the previous one
     stage();
+    if (OUT) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int m = 0; m < MS; ++m) dec_store4(stile + (scol + 16 * m + l16) * PK + srow + 16 * t + 4 * g, S[t][m]);
+    }
     __syncthreads();
     if (t0 + C < end) fetch(t0 + C);
 
-    if (t0 == s0 || n < C) {  // lambda^(n-1-j) of this lane's contraction indices (frames behind the end hold zeros)
+    if (OUT && 16 * it < n) {
+      Frag qx[KB];
 #pragma unroll
-      for (int jb = 0; jb < JB; ++jb)
+      for (int kb = 0; kb < KB; ++kb) dec_lds_frag(qx[kb], qtile + (16 * it + l16) * PK + kb * 32 + g * 8);
+      dec_f4 o[MO];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) wv[jb][e] = dec_pow(a2, max(n - 1 - (jb * 32 + (e >> 2) * 16 + 4 * g + (e & 3)), 0));
-    }
-    Frag vt[MT][JB];  // V^T: row = column of v, contraction over frames
+      for (int i = 0; i < MO; ++i) {  // column tile mo: columns 32 (mo / 2) + 4 (mo % 2) + 8 (row / 4) + row % 4
+        const int mo = mo0 + i;
+        const T* const sr = stile + (32 * (mo >> 1) + 4 * (mo & 1) + 8 * (l16 >> 2) + (l16 & 3)) * PK + g * 8;
+        o[i] = dec_f4(0.f);
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int jb = 0; jb < JB; ++jb) dec_lds_frag(vt[m][jb], vcol + (col0 + 16 * m + l16) * G::PC + jb * 32 + g * 8);
-
-    if (OUT) {
-      Frag st[MT][KB];  // S^T
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) dec_pack(st[m][kb], S[2 * kb][m], S[2 * kb + 1][m]);
-#pragma unroll
-      for (int it = 0; it < IT; ++it) {
-        Frag qx[KB];
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) dec_lds_frag(qx[kb], qrow + (16 * it + l16) * G::PR + kb * 32 + g * 8);
-        dec_f4 o[MT];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          o[m] = dec_f4(0.f);
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb) o[m] = dec_mma(st[m][kb], qx[kb], o[m]);
-          o[m] *= fq[it];
+        for (int kb = 0; kb < KB; ++kb) {
+          Frag sx;
+          dec_lds_frag(sx, sr + kb * 32);
+          o[i] = dec_mma(sx, qx[kb], o[i]);
         }
+        o[i] *= fq;
+      }
+#pragma unroll 1
+      for (int jb = 0; jb <= it >> 1; ++jb) {
+        dec_f4 p[2];
 #pragma unroll
-        for (int jb = 0; jb <= it / 2; ++jb) {
-          dec_f4 p[2];
+        for (int x = 0; x < 2; ++x) {
+          const int jt = 2 * jb + x;
+          p[x] = dec_f4(0.f);
+          if (jt > it) continue;
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int jt = 2 * jb + x;
-            p[x] = dec_f4(0.f);
-            if (jt > it) continue;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-              Frag kx;
-              dec_lds_frag(kx, krow + (16 * jt + l16) * G::PR + kb * 32 + g * 8);
-              p[x] = dec_mma(kx, qx[kb], p[x]);
-            }
-            if (jt == it) {  // masked by selection: a frame behind this one contributes nothing, whatever it holds
-#pragma unroll
-              for (int r = 0; r < 4; ++r) p[x][r] = l16 >= 4 * g + r ? p[x][r] * wdiag[r] : 0.f;
-            } else {
-#pragma unroll
-              for (int r = 0; r < 4; ++r) p[x][r] *= woff[r] * wfar[it - jt];
-            }
+          for (int kb = 0; kb < KB; ++kb) {
+            Frag kx;
+            dec_lds_frag(kx, ktile + (16 * jt + l16) * PK + kb * 32 + g * 8);
+            p[x] = dec_mma(kx, qx[kb], p[x]);
           }
-          Frag pf;
-          dec_pack(pf, p[0], p[1]);
+          if (jt == it) {  // masked by selection: a frame behind this one contributes nothing, whatever it holds
 #pragma unroll
-          for (int m = 0; m < MT; ++m) o[m] = dec_mma(vt[m][jb], pf, o[m]);
+            for (int r = 0; r < 4; ++r) p[x][r] = l16 >= 4 * g + r ? p[x][r] * wdiag[r] : 0.f;
+          } else {
+            const float far = upow(16 * (it - jt - 1));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) p[x][r] *= woff[r] * far;
+          }
         }
-        const int t = t0 + 16 * it + l16;
-        if (t < end) {
-          T* dst = op + (long)(rev ? len - 1 - t : t) * R.out.ld + 4 * g;
+        Frag pf;
+        dec_pack(pf, p[0], p[1]);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) dec_store4(dst + 16 * m, o[m] * args.scale);
+        for (int i = 0; i < MO; ++i) {
+          const int mo = mo0 + i;
+          Frag vx;
+          dec_cols_spread<PV>(vx, vtile + jb * 32 * PV + 32 * (mo >> 1) + 4 * (mo & 1), l16, g);
+          o[i] = dec_mma(vx, pf, o[i]);
+        }
+      }
+      const int t = t0 + 16 * it + l16;
+      if (t < end) {
+        T* const dst = op + (long)(rev ? len - 1 - t : t) * R.out.ld;
+        if constexpr (MO == 1) {
+          dec_store4(dst + 32 * (mo0 >> 1) + 4 * (mo0 & 1), o[0] * args.scale);
+        } else {
+#pragma unroll
+          for (int i = 0; i < MO; i += 2) dec_store8(dst + 16 * (mo0 + i), o[i] * args.scale, o[i + 1] * args.scale);
         }
       }
     }
 
     // ---- the state behind the chunk
-    const float lam = dec_pow(a2, n);
+    const float lam = upow(n);
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int m = 0; m < MT; ++m) S[t][m] *= lam;
+      for (int m = 0; m < MS; ++m) S[t][m] *= lam;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int jb = 0; jb < JB; ++jb) {
+      float w[8];  // lambda^(n-1-j) of this lane's frames (those behind the end hold zeros)
+      if (n == C) {
+        const float w0 = upow(C - 16 - 32 * jb), w1 = upow(C - 32 - 32 * jb);
 #pragma unroll
-      for (int jb = 0; jb < JB; ++jb) {
+        for (int e = 0; e < 4; ++e) w[e] = wend[e] * w0, w[4 + e] = wend[e] * w1;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = dec_pow(a2, max(n - 1 - (jb * 32 + (e >> 2) * 16 + 4 * g + (e & 3)), 0));
+      }
+      Frag wv[MS][sizeof(T) == 2 ? TERMS : 1];
+#pragma unroll
+      for (int m = 0; m < MS; ++m) {
+        Frag vx;
+        dec_cols<PV>(vx, vtile + jb * 32 * PV + scol + 16 * m, l16, g);
         if constexpr (sizeof(T) == 2) {
-          dec_b8 s[3];
-          dec_split(vt[m][jb], wv[jb], s);
-#pragma unroll
-          for (int t = 0; t < KT; ++t) {
-            Frag kx;
-            dec_lds_frag(kx, kcol + (16 * t + l16) * G::PC + jb * 32 + g * 8);
-#pragma unroll
-            for (int x = 2; x >= 0; --x) S[t][m] = dec_mma(kx, s[x], S[t][m]);
-          }
+          dec_split<TERMS>(vx, w, wv[m]);
         } else {
-          Frag s;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s.a[e] = vt[m][jb].a[e] * wv[jb][e], s.b[e] = vt[m][jb].b[e] * wv[jb][4 + e];
-#pragma unroll
-          for (int t = 0; t < KT; ++t) {
-            Frag kx;
-            dec_lds_frag(kx, kcol + (16 * t + l16) * G::PC + jb * 32 + g * 8);
-            S[t][m] = dec_mma(kx, s, S[t][m]);
-          }
+          for (int e = 0; e < 4; ++e) wv[m][0].a[e] = vx.a[e] * w[e], wv[m][0].b[e] = vx.b[e] * w[4 + e];
         }
       }
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        Frag kx;
+        dec_cols<PK>(kx, ktile + jb * 32 * PK + srow + 16 * t, l16, g);
+#pragma unroll
+        for (int m = 0; m < MS; ++m)
+#pragma unroll
+          for (int x = (sizeof(T) == 2 ? TERMS : 1) - 1; x >= 0; --x) S[t][m] = dec_mma(kx, wv[m][x], S[t][m]);
+      }
+    }
   }
 
   if (!OUT) {
-    dec_f4* e = reinterpret_cast<dec_f4*>(R.ws + ((long)bh * args.segments + seg) * (DK * DV)) + wave * (KT * MT * 64) + lane;
+    dec_f4* e = reinterpret_cast<dec_f4*>(R.ws + ((long)bh * args.segments + seg) * (DK * DV)) + wplace;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int m = 0; m < MT; ++m) e[(t * MT + m) * 64] = S[t][m];
+      for (int m = 0; m < MS; ++m) e[(t * MS + m) * 64] = S[t][m];
     return;
   }
   // zeros behind the utterance's end
@@ -450,37 +488,43 @@ __global__ __launch_bounds__(64 * (DV >= 64 ? 4 : 2)) void k_decay(DecayArgs arg
   }
   // the final state, by the segment that holds the last frame (an empty utterance keeps what it had)
   if (args.state && s0 < len && s1 >= len) {
-    float* sp = args.state + (long)bh * DK * DV;
+    float* sp = args.state + (long)bh * DK * DV + splace;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MS; ++m)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sp[(16 * t + 4 * g + r) * DV + col0 + 16 * m + l16] = S[t][m][r];
+        for (int r = 0; r < 4; ++r) sp[(16 * t + r) * DV + 16 * m] = S[t][m][r];
   }
 }
 
-template <class T, int DK, int DV>
-static int decay_launch(const DecayArgs& a, int roles, hipStream_t st) {
+template <class T, int DK, int DV, int TERMS>
+static int decay_launch_terms(const DecayArgs& a, int roles, hipStream_t st) {
   typedef DecGeo<T, DK, DV> G;
   static_assert(G::kLdsOut <= 160 * 1024, "a workgroup's tiles fit the CU's LDS");
-  if (G::kLdsOut > 64 * 1024) {  // above the default limit of dynamic LDS
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_decay<T, DK, DV, true>),
+  if (G::kLdsOut > 48 * 1024) {  // more dynamic LDS than the default limit has to be asked for
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_decay<T, DK, DV, true, TERMS>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)G::kLdsOut);
     if (e != hipSuccess) return set_error("decay attention: %zu bytes of LDS refused: %s", G::kLdsOut, hipGetErrorString(e));
   }
   if (a.segments > 1) {
     ProfScope ps("k_decay_states", st);
-    hipLaunchKernelGGL((k_decay<T, DK, DV, false>), dim3(a.B * a.H, a.segments - 1, roles), dim3(G::THREADS), G::kLdsState,
-                       st, a);
+    hipLaunchKernelGGL((k_decay<T, DK, DV, false, TERMS>), dim3(a.B * a.H, a.segments - 1, roles), dim3(G::THREADS),
+                       G::kLdsState, st, a);
   }
   {
     ProfScope ps("k_decay", st);
-    hipLaunchKernelGGL((k_decay<T, DK, DV, true>), dim3(a.B * a.H, a.segments, roles), dim3(G::THREADS), G::kLdsOut, st, a);
+    hipLaunchKernelGGL((k_decay<T, DK, DV, true, TERMS>), dim3(a.B * a.H, a.segments, roles), dim3(G::THREADS), G::kLdsOut,
+                       st, a);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error("launch of k_decay failed: %s", hipGetErrorString(e));
   return 0;
+}
+template <class T, int DK, int DV>
+static int decay_launch(const DecayArgs& a, int roles, hipStream_t st) {
+  if constexpr (sizeof(T) == 4) return decay_launch_terms<T, DK, DV, 1>(a, roles, st);
+  else return a.state ? decay_launch_terms<T, DK, DV, 3>(a, roles, st) : decay_launch_terms<T, DK, DV, 2>(a, roles, st);
 }
 
 #define DECAY_FOR_WIDTHS(T, DK_, DV_, RESULT, EXPR)                        \

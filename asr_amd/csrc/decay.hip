@@ -57,6 +57,53 @@ __global__ __launch_bounds__(kDecayStepThreads) void k_decay_step(const T* __res
   }
 }
 
+// k_decay_join: a workgroup takes 64 places (16 bytes each) of one head's states, its sixteen waves up to eight consecutive
+// segments each, read at once.  A wave first sums its own, the waves' sums meet in LDS.  (Summed by every segment's workgroup for
+// itself instead, 62 segments of one head cost 24 us of reads.)
+constexpr int kJoinEach = kDecayMaxSegments / 16;
+__global__ __launch_bounds__(1024) void k_decay_join(float* ws, long role_stride, const float* __restrict__ log_decay,
+                                                     const int* __restrict__ lengths, int T, int H, int segments, int seg_len,
+                                                     int places) {
+  __shared__ dec_f4 sum[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bh = blockIdx.x, b = bh / H;
+  const int len = lengths ? min(max(lengths[b], 0), T) : T;
+  const int have = min(segments - 1, len > 0 ? (len - 1) / seg_len : 0);  // segments that another one follows left a state
+  const int per = (segments - 1 + 15) / 16, from = wave * per, n = min(per, have - from);
+  dec_f4* const e = reinterpret_cast<dec_f4*>(ws + blockIdx.z * role_stride) + ((long)bh * segments + from) * places + blockIdx.y * 64 + lane;
+  const float a2 = dec_log2(log_decay[bh - b * H]), lam = dec_pow(a2, seg_len);
+  dec_f4 x[kJoinEach], acc = dec_f4(0.f);
+  if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < kJoinEach; ++i) x[i] = e[(long)min(i, n - 1) * places];
+#pragma unroll
+    for (int i = 0; i < kJoinEach; ++i)
+      if (i < n) acc = lam * acc + x[i];
+  }
+  sum[wave][lane] = acc;
+  __syncthreads();
+  if (n <= 0) return;
+  // (the waves before this one are full)
+  const float lam_per = dec_pow(a2, per * seg_len);
+  acc = dec_f4(0.f);
+#pragma unroll 4
+  for (int w = 0; w < wave; ++w) acc = lam_per * acc + sum[w][lane];
+#pragma unroll
+  for (int i = 0; i < kJoinEach; ++i)
+    if (i < n) {
+      acc = lam * acc + x[i];
+      e[(long)i * places] = acc;
+    }
+}
+
+int decay_launch_join(const DecayArgs& a, int roles, int state_elements, hipStream_t st) {
+  ProfScope ps("k_decay_join", st);
+  const long stride = roles > 1 ? a.role[1].ws - a.role[0].ws : 0;
+  hipLaunchKernelGGL(k_decay_join, dim3(a.B * a.H, state_elements / 256, roles), dim3(1024), 0, st, a.role[0].ws, stride,
+                     a.log_decay, a.lengths, a.T, a.H, a.segments, a.seg_len, state_elements / 4);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : set_error("launch of k_decay_join failed: %s", hipGetErrorString(e));
+}
+
 static bool decay_width(int d) { return d == 32 || d == 64 || d == 128; }
 
 static int decay_check(const char* what, int dtype, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv) {
@@ -67,13 +114,15 @@ static int decay_check(const char* what, int dtype, int32_t B, int32_t T, int32_
   return 0;
 }
 
-// Segments an utterance's frames are split into: enough workgroups to fill the chip when there are few heads in all.
-// A split costs a second read of k and v and a launch.
-static int decay_segments(int dtype, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int* seg_len) {
+// Segments an utterance's frames are split into when there are few heads in all: one workgroup walks a chunk in 1.5 us, and
+// about 200 of them saturate the memory.  A split costs a second read of k and v and a launch, from kDecayJoinFrom segments on
+// another one.  Measured, whole call: 6 heads of 23999 frames bf16 in 46 segments 42.6 us, in 124 37.7 us; 96 heads of 400 frames
+// f32 in 2 segments 31.1 us, in 3 27.9 us, in 5 34.0 us; 192 heads of 3000 frames bf16 whole 74 us, in 2 90 us, in 4 78 us.
+static int decay_segments(int dtype, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int roles, int* seg_len) {
   const int chunk = dtype == LMUFFT_BF16 ? decay_chunk_bf16(dk, dv) : decay_chunk_f32(dk, dv);
-  const long heads = (long)B * H, chunks = std::max<long>(1, (T + (long)chunk - 1) / chunk);
-  long n = std::min<long>(std::min<long>(kDecayMaxSegments, 1024 / std::max<long>(1, heads)), chunks / 2);
-  n = std::max<long>(n, 1);
+  const long heads = std::max<long>(1, (long)B * H * roles), chunks = std::max<long>(1, (T + (long)chunk - 1) / chunk);
+  long n = std::min<long>((heads <= 16 ? 768 : 320) / heads, chunks / 2);  // (no segment of a single chunk)
+  n = std::max<long>(std::min<long>(n, kDecayMaxSegments), 1);
   const long per = (chunks + n - 1) / n;
   *seg_len = (int)(per * chunk);
   return (int)((chunks + per - 1) / per);
@@ -108,7 +157,7 @@ extern "C" size_t lmufft_decay_workspace_bytes(int dtype, int32_t B, int32_t T, 
                                                int backward) {
   if (decay_check("decay attention", dtype, B, T, H, dk, dv)) return 0;
   int seg_len = 0;
-  const int n = decay_segments(dtype, B, T, H, dk, dv, &seg_len);
+  const int n = decay_segments(dtype, B, T, H, dk, dv, backward ? 3 : 1, &seg_len);
   return n > 1 ? sizeof(float) * (backward ? 3 : 1) * (size_t)B * H * n * dk * dv : 0;
 }
 
@@ -129,7 +178,7 @@ extern "C" int lmufft_decay_attention(const void* q, const void* k, const void* 
     return 1;
   if (!log_decay) return set_error("%s: `log_decay` is NULL", what);
   if (reinterpret_cast<uintptr_t>(state) & 15) return set_error("%s: `state` must be 16-byte aligned", what);
-  a.segments = decay_segments(dtype, B, T, H, dk, dv, &a.seg_len);
+  a.segments = decay_segments(dtype, B, T, H, dk, dv, 1, &a.seg_len);
   const size_t need = lmufft_decay_workspace_bytes(dtype, B, T, H, dk, dv, 0);
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return set_error("%s: workspace of %zu bytes on a 16-byte boundary needed, %zu given", what, need, workspace_bytes);
@@ -139,6 +188,7 @@ extern "C" int lmufft_decay_attention(const void* q, const void* k, const void* 
   a.state = state;
   a.scale = scale;
   a.B = B, a.T = T, a.H = H;
+  a.joined = a.segments >= kDecayJoinFrom;
   return decay_launch_any(dtype, a, 1, dk, dv, (hipStream_t)stream);
 }
 
@@ -163,7 +213,7 @@ extern "C" int lmufft_decay_attention_bwd(const void* q, const void* k, const vo
     return 1;
   if (!log_decay) return set_error("%s: `log_decay` is NULL", what);
   DecayArgs a{};
-  a.segments = decay_segments(dtype, B, T, H, dk, dv, &a.seg_len);
+  a.segments = decay_segments(dtype, B, T, H, dk, dv, 3, &a.seg_len);
   const size_t need = lmufft_decay_workspace_bytes(dtype, B, T, H, dk, dv, 1);
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return set_error("%s: workspace of %zu bytes on a 16-byte boundary needed, %zu given", what, need, workspace_bytes);
@@ -171,6 +221,7 @@ extern "C" int lmufft_decay_attention_bwd(const void* q, const void* k, const vo
   a.lengths = lengths;
   a.scale = scale;
   a.B = B, a.T = T, a.H = H;
+  a.joined = a.segments >= kDecayJoinFrom;
   const size_t part = (size_t)B * H * a.segments * dk * dv;
   float* const ws = (float*)workspace;
   // dq = A(do, v, k); dk = A_reversed(v, do, q); dv = A_reversed(k, q, do): one launch when the head widths agree

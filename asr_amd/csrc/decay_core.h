@@ -11,17 +11,20 @@
 //   dq = A(do, v, k),   dk = A_reversed(v, do, q),   dv = A_reversed(k, q, do),
 // so one kernel serves both directions and a launch takes up to three such roles.
 //
-// A workgroup of four waves owns one (utterance, head, segment of frames) and walks the segment's chunks.  For the outputs
-// a wave owns sixteen frames of the chunk (and, in chunks of 32, half of the columns); the state is held as MFMA accumulators,
-// its tiles split over the waves.  With transposed products a wave's intermediates stay in its registers, because the
-// accumulator layout of a 16 x 16 tile (lane = column, four consecutive rows) is, two tiles side by side, the operand layout
-// of the next product up to a permutation of the contraction index, which the reads of the other operand follow:
+// A workgroup of eight waves owns one (utterance, head, segment of frames) and walks the segment's chunks.  Four waves make
+// the outputs, each of sixteen frames of the chunk (in chunks of 32, of half of the columns); four hold the state as MFMA
+// accumulators, its tiles split between them, and bring it behind the chunk meanwhile -- the two halves of a chunk are
+// independent, and side by side the chain of a chunk is half as long.  With transposed products a wave's intermediates stay
+// in its registers, because the accumulator layout of a 16 x 16 tile (lane = column, four consecutive rows) is, two tiles side
+// by side, the operand layout of the next product up to a permutation of the contraction index, which the reads of the other
+// operand follow:
 //   P^T = K Q^T          A = K rows, B = Q rows
 //   O^T = S^T Q^T + V^T P^T     A = S^T rows, B = Q rows;  A = V^T columns, B = P^T's accumulators
 //   S  += K^T (w V)      A = K^T columns, B = V^T columns scaled by lambda^(C-1-j)
 // q, k, v go through LDS by rows, as they lie in memory, and the state in the products' type; columns are read from there by
-// the transposing LDS read (bf16) or element by element (f32).  The next chunk's rows are fetched into registers while the
-// present one is computed, and the state is handed over at the barriers that the tiles need anyway.
+// the transposing LDS read (bf16) or element by element (f32).  Rows are stored without padding, their 16-byte pieces in an
+// order that depends on the row, so that writes, row and column reads all spread over the banks (DecTile).  The next chunk's
+// rows are fetched into registers while the present one is computed.
 //
 // Rounding: products accumulate in 32 bits and the state is held in 32 bits.  bf16 tensors: P and the copy of S that
 // multiplies q are rounded to bf16 once (what a bf16 operand of the matrix cores costs; each is below the rounding of the
@@ -42,7 +45,8 @@ typedef __bf16 dec_b8 __attribute__((ext_vector_type(8)));
 typedef __bf16 dec_b4 __attribute__((ext_vector_type(4)));
 typedef unsigned int dec_u4 __attribute__((ext_vector_type(4)));
 
-constexpr int kDecayMaxSegments = 32;
+constexpr int kDecayMaxSegments = 128;
+constexpr int kDecayJoinFrom = 5;  // segments from which on their states are joined by a launch of its own
 constexpr int kDecayMaxRoles = 3;
 
 // One tensor [B][T][H * width] with unit column stride: element strides of a frame and of an utterance.
@@ -62,7 +66,7 @@ struct DecayArgs {
   const int* lengths;      // [B] or NULL
   float* state;            // [B][H][DK][DV]: read at the start, replaced at the end; or NULL
   float scale;
-  int B, T, H, segments, seg_len;
+  int B, T, H, segments, seg_len, joined;
 };
 
 int decay_chunk_bf16(int dk, int dv);  // frames per chunk
@@ -105,11 +109,6 @@ __device__ __forceinline__ void dec_pack(DecTraits<float>::frag& f, const dec_f4
   f.a = lo;
   f.b = hi;
 }
-__device__ __forceinline__ void dec_lds_frag(dec_b8& f, const __bf16* p) { f = *reinterpret_cast<const dec_b8*>(p); }
-__device__ __forceinline__ void dec_lds_frag(DecTraits<float>::frag& f, const float* p) {
-  f.a = *reinterpret_cast<const dec_f4*>(p);
-  f.b = *reinterpret_cast<const dec_f4*>(p + 4);
-}
 __device__ __forceinline__ void dec_store4(__bf16* p, const dec_f4& v) {
   dec_b4 o;
 #pragma unroll
@@ -117,15 +116,57 @@ __device__ __forceinline__ void dec_store4(__bf16* p, const dec_f4& v) {
   *reinterpret_cast<dec_b4*>(p) = o;
 }
 __device__ __forceinline__ void dec_store4(float* p, const dec_f4& v) { *reinterpret_cast<dec_f4*>(p) = v; }
-__device__ __forceinline__ void dec_store8(__bf16* p, const dec_f4& v, const dec_f4& w) {
-  dec_b8 o;
-  dec_pack(o, v, w);
-  *reinterpret_cast<dec_b8*>(p) = o;
-}
-__device__ __forceinline__ void dec_store8(float* p, const dec_f4& v, const dec_f4& w) {
-  dec_store4(p, v);
-  dec_store4(p + 4, w);
-}
+
+// A tile of rows of D elements in LDS.  Sixteen 16-byte pieces lie side by side over the banks: the pieces of a row are stored
+// at their place xor a key of the row, such that one piece of sixteen consecutive rows (the row reads), and two neighbouring
+// pieces of eight (the column reads, 32 lanes at a time), all lie apart.
+template <class T, int D>
+struct DecTile {
+  typedef typename DecTraits<T>::frag Frag;
+  static constexpr int VEC = DecTraits<T>::kVec, NP = D / VEC, RP = NP < 16 ? 16 / NP : 1, KEYS = NP < 16 ? NP : 16;
+  T* base;
+  static __device__ __forceinline__ int key(int row) {  // the row's number among those that would collide, its top bit last
+    const int k = row / RP % KEYS;
+    return (2 * k + 2 * k / KEYS) % KEYS;
+  }
+  __device__ __forceinline__ T* piece(int row, int p) const { return base + row * D + (p ^ key(row)) * VEC; }
+  // eight elements of a row from column 32 kb + 8 g on
+  __device__ __forceinline__ Frag row_frag(int row, int kb, int g) const {
+    Frag f;
+    if constexpr (VEC == 8) {
+      f = *reinterpret_cast<const dec_b8*>(piece(row, 4 * kb + g));
+    } else {
+      f.a = *reinterpret_cast<const dec_f4*>(piece(row, 8 * kb + 2 * g));
+      f.b = *reinterpret_cast<const dec_f4*>(piece(row, 8 * kb + 2 * g + 1));
+    }
+    return f;
+  }
+  // column c0 + l16 of the rows r0 + 4g..4g+3 and r0 + 16+4g..16+4g+3, as the accumulators of two tiles hold them (c0, r0
+  // multiples of sixteen).  The transposing read: of sixteen lanes, lane 4 q + p addresses four columns, piece p, of row q, and
+  // lane i receives the four rows' values of the i-th of the sixteen columns.
+  __device__ __forceinline__ Frag col_frag(int r0, int c0, int l16, int g) const {
+    Frag f;
+    if constexpr (VEC == 8) {
+      typedef dec_b4 __attribute__((address_space(3))) * lds4;
+      const int row = 4 * g + (l16 >> 2);
+      const T* const a = base + (r0 + row) * D + ((c0 / 8 + ((l16 >> 1) & 1)) ^ key(row)) * 8 + (l16 & 1) * 4;
+      const dec_b4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)a);
+      const dec_b4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(a + 16 * D));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = lo[e], f[4 + e] = hi[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const T* const a = piece(4 * g + e, c0 / 4 + (l16 >> 2)) + r0 * D + (l16 & 3);
+        f.a[e] = a[0];
+        f.b[e] = a[16 * D];
+      }
+    }
+    return f;
+  }
+  // four elements of a row from a column that is a multiple of four
+  __device__ __forceinline__ void put4(int row, int c, const dec_f4& v) const { dec_store4(piece(row, c / VEC) + c % VEC, v); }
+};
 
 // lambda^n for n >= 0 from log2 lambda, which is held above -2^100 so that lambda = 0 gives lambda^0 = 1 (and 0 behind it)
 __device__ __forceinline__ float dec_log2(float log_decay) {
@@ -135,39 +176,6 @@ __device__ __forceinline__ float dec_log2(float log_decay) {
 __device__ __forceinline__ float dec_pow(float a2, int n) { return __builtin_amdgcn_exp2f(a2 * (float)n); }
 __device__ __forceinline__ float dec_uniform(float x) {
   return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x)));
-}
-
-// Column fragments of a tile that lies in LDS by rows (pitch P): a lane's eight values are one column of the rows 4g..4g+3 and
-// 16+4g..16+4g+3 behind `tile`, as the accumulators of two tiles hold them.  Lane i of sixteen has the column i.
-// dec_cols_spread: it has the column 8 (i / 4) + i % 4 (of 32; the other sixteen lie four columns on): the accumulators of two
-// such tiles hold eight columns side by side.
-template <int P>
-__device__ __forceinline__ void dec_cols_at(dec_b8& f, const __bf16* a) {
-  typedef dec_b4 __attribute__((address_space(3))) * lds4;
-  const dec_b4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)a);
-  const dec_b4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(a + 16 * P));
-#pragma unroll
-  for (int e = 0; e < 4; ++e) f[e] = lo[e], f[4 + e] = hi[e];
-}
-// (the transposing read: of sixteen lanes, lane 4 q + p addresses four columns, piece p, of row q; lane i receives the four
-// rows' values of the i-th column of the four pieces side by side)
-template <int P>
-__device__ __forceinline__ void dec_cols(dec_b8& f, const __bf16* tile, int l16, int g) {
-  dec_cols_at<P>(f, tile + (4 * g + (l16 >> 2)) * P + 4 * (l16 & 3));
-}
-template <int P>
-__device__ __forceinline__ void dec_cols_spread(dec_b8& f, const __bf16* tile, int l16, int g) {
-  dec_cols_at<P>(f, tile + (4 * g + (l16 >> 2)) * P + 8 * (l16 & 3));
-}
-template <int P>
-__device__ __forceinline__ void dec_cols(DecTraits<float>::frag& f, const float* tile, int l16, int g) {
-  const float* a = tile + 4 * g * P + l16;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) f.a[e] = a[e * P], f.b[e] = a[(16 + e) * P];
-}
-template <int P>
-__device__ __forceinline__ void dec_cols_spread(DecTraits<float>::frag& f, const float* tile, int l16, int g) {
-  dec_cols<P>(f, tile, 8 * (l16 >> 2) + (l16 & 3), g);
 }
 
 // w v in TERMS bf16 terms: what is left behind the last is below 2^(-9 TERMS) of the value
@@ -189,39 +197,40 @@ template <class T, int DK, int DV>
 struct DecGeo {
   // frames per chunk: 64, or 32 where the tiles would leave room for one workgroup a CU, and for f32, whose products cost more
   static constexpr int C = sizeof(T) == 2 && DK + DV < 256 ? 64 : 32;
-  static constexpr int THREADS = 256;
-  static constexpr int WQ = C / 16, WD = 4 / WQ;      // waves over the chunk's frames, over the columns of the outputs
+  static constexpr int WQ = C / 16, WD = 4 / WQ;      // output waves over the chunk's frames, over the columns
   static constexpr int MO = DV / 16 / WD;             // column tiles of a wave's outputs
   static constexpr int MS = DV >= 64 ? DV / 64 : 1;   // column tiles of a wave's part of the state
   static constexpr int KS = DV >= 64 ? 1 : 2;         // waves over the rows of the state
   static constexpr int KT = DK / 16 / KS;             // row tiles of a wave's part
-  static constexpr int PAD = 16 / sizeof(T);          // rows 16 bytes longer than their data: sixteen rows hit different banks
-  static constexpr int PK = DK + PAD, PV = DV + PAD;  // pitches of the k, q and state tiles, and of the v tile
   static constexpr int VEC = DecTraits<T>::kVec;
-  static constexpr int NK = C * DK / VEC / THREADS, NV = C * DV / VEC / THREADS;  // 16-byte pieces a thread stages
-  static_assert(NK * VEC * THREADS == C * DK && NV * VEC * THREADS == C * DV, "whole pieces for every thread");
-  static constexpr size_t kLdsState = sizeof(T) * (size_t)C * (PK + PV);
-  static constexpr size_t kLdsOut = kLdsState + sizeof(T) * (size_t)(C + DV) * PK;
-  static constexpr int WAVES = kLdsOut <= 52 * 1024 ? 3 : 2;  // a SIMD: as many workgroups as the LDS holds, and no spills
+  static constexpr size_t kLdsState = sizeof(T) * (size_t)C * (DK + DV);
+  static constexpr size_t kLdsOut = kLdsState + sizeof(T) * (size_t)(C + DV) * DK;
+  static constexpr int WAVES = kLdsOut <= 40 * 1024 && DV <= 64 ? 4 : 2;  // a SIMD: two workgroups of eight waves a CU, or one
 };
 
-// OUT: the outputs and, in the last segment, the final state.  !OUT: the states at the ends of all segments but the
-// last (which the OUT kernel joins), from zero or, in the first segment, from the initial state.
+// OUT (eight waves): the outputs and, in the last segment, the final state.  !OUT (the four waves of the state alone): the
+// states at the ends of all segments but the last (which the OUT kernel joins), from zero or, in the first segment, from the
+// initial state.
 // TERMS: bf16 terms of the scaled v that enters the state (see above): three where the state is returned, two where it only
 // serves outputs that are rounded to bf16 themselves.
 template <class T, int DK, int DV, bool OUT, int TERMS>
-__global__ __launch_bounds__(256, (DecGeo<T, DK, DV>::WAVES)) void k_decay(DecayArgs args) {
+__global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k_decay(DecayArgs args) {
   typedef DecGeo<T, DK, DV> G;
   typedef typename DecTraits<T>::frag Frag;
-  constexpr int C = G::C, MS = G::MS, KT = G::KT, MO = G::MO, KB = DK / 32, JB = C / 32, VEC = G::VEC, PK = G::PK, PV = G::PV;
+  constexpr int THREADS = OUT ? 512 : 256;
+  constexpr int C = G::C, MS = G::MS, KT = G::KT, MO = G::MO, KB = DK / 32, JB = C / 32, VEC = G::VEC;
+  constexpr int PIECES_K = C * DK / VEC, PIECES_V = C * DV / VEC;  // 16-byte pieces of the tiles, and how many a thread stages
+  constexpr int NK = (PIECES_K + THREADS - 1) / THREADS, NV = (PIECES_V + THREADS - 1) / THREADS;
   extern __shared__ __attribute__((aligned(16))) unsigned char dec_lds[];
-  T* const ktile = reinterpret_cast<T*>(dec_lds);  // [C][DK]
-  T* const vtile = ktile + C * PK;                 // [C][DV]
-  T* const qtile = vtile + C * PV;                 // [C][DK]
-  T* const stile = qtile + C * PK;                 // [DV][DK]: S^T
+  const DecTile<T, DK> ktile{reinterpret_cast<T*>(dec_lds)};  // [C][DK]
+  const DecTile<T, DV> vtile{ktile.base + C * DK};            // [C][DV]
+  const DecTile<T, DK> qtile{vtile.base + C * DV};            // [C][DK]
+  const DecTile<T, DK> stile{qtile.base + C * DK};            // [DV][DK]: S^T
 
   const DecayRole& R = args.role[blockIdx.z];
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;             // among those of its kind
+  const bool holds = !OUT || __builtin_amdgcn_readfirstlane(tid >> 8) != 0;  // a wave of the state
   const int bh = blockIdx.x, b = bh / args.H, h = bh - b * args.H, seg = blockIdx.y;
   const int T_ = args.T;
   const int len = args.lengths ? min(max(args.lengths[b], 0), T_) : T_;
@@ -229,7 +238,7 @@ __global__ __launch_bounds__(256, (DecGeo<T, DK, DV>::WAVES)) void k_decay(Decay
   const int end = min(s1, len);  // frames s0..end-1 are computed, end..s1-1 (of the padding) get zeros
   const bool first = s0 == 0, single = args.segments == 1;
   const bool rev = R.reverse != 0;
-  // this wave's part of the state: rows srow.., columns scol..; and of the outputs: frames 16 it.., column tiles mo0..
+  // this wave's part of the state: rows srow.., columns scol..; or of the outputs: frames 16 it.., column tiles mo0..
   const int srow = G::KS == 1 ? 0 : (wave >> 1) * KT * 16, scol = G::KS == 1 ? wave * MS * 16 : (wave & 1) * 16;
   const int it = wave % G::WQ, mo0 = wave / G::WQ * MO;
 
@@ -238,7 +247,7 @@ __global__ __launch_bounds__(256, (DecGeo<T, DK, DV>::WAVES)) void k_decay(Decay
     if (first && args.state) {
       const float* src = args.state + (long)bh * DK * DV;
       float* dst = R.ws + ((long)bh * args.segments + args.segments - 1) * (DK * DV);
-      for (int i = tid * 4; i < DK * DV; i += G::THREADS * 4)
+      for (int i = tid * 4; i < DK * DV; i += THREADS * 4)
         *reinterpret_cast<dec_f4*>(dst + i) = *reinterpret_cast<const dec_f4*>(src + i);
     }
     if (s0 + args.seg_len >= len) return;  // nobody needs the state behind this segment
@@ -250,141 +259,106 @@ __global__ __launch_bounds__(256, (DecGeo<T, DK, DV>::WAVES)) void k_decay(Decay
     return reinterpret_cast<const char*>(x.p) + ((long)b * x.bs + (long)h * width) * (long)sizeof(T);
   };
   const char *const kbase = head(R.k, DK), *const vbase = head(R.v, DV), *const qbase = OUT ? head(R.q, DK) : nullptr;
-  unsigned koff[G::NK], qoff[OUT ? G::NK : 1], voff[G::NV];
+  auto krow = [&](int n) { return (tid + n * THREADS) / (DK / VEC); };
+  auto kpiece = [&](int n) { return (tid + n * THREADS) % (DK / VEC); };
+  auto vrow = [&](int n) { return (tid + n * THREADS) / (DV / VEC); };
+  auto vpiece = [&](int n) { return (tid + n * THREADS) % (DV / VEC); };
+  auto offset = [&](int row, int p, long ld) {
+    return ((unsigned)(rev ? C - 1 - row : row) * (unsigned)ld + (unsigned)(p * VEC)) * (unsigned)sizeof(T);
+  };
+  unsigned koff[NK], qoff[OUT ? NK : 1], voff[NV];
 #pragma unroll
-  for (int n = 0; n < G::NK; ++n) {
-    const int u = tid + n * G::THREADS, row = u / (DK / VEC), c = u % (DK / VEC) * VEC, m = rev ? C - 1 - row : row;
-    koff[n] = (unsigned)((m * R.k.ld + c) * (long)sizeof(T));
-    if (OUT) qoff[n] = (unsigned)((m * R.q.ld + c) * (long)sizeof(T));
+  for (int n = 0; n < NK; ++n) {
+    koff[n] = offset(krow(n), kpiece(n), R.k.ld);
+    if (OUT) qoff[n] = offset(krow(n), kpiece(n), R.q.ld);
   }
 #pragma unroll
-  for (int n = 0; n < G::NV; ++n) {
-    const int u = tid + n * G::THREADS, row = u / (DV / VEC), c = u % (DV / VEC) * VEC, m = rev ? C - 1 - row : row;
-    voff[n] = (unsigned)((m * R.v.ld + c) * (long)sizeof(T));
-  }
-  dec_u4 kf[G::NK], qf[G::NK], vf[G::NV];
-  auto fetch = [&](int t0) {
+  for (int n = 0; n < NV; ++n) voff[n] = offset(vrow(n), vpiece(n), R.v.ld);
+  struct Rows {  // a chunk's pieces on their way from memory
+    dec_u4 k[NK], q[OUT ? NK : 1], v[NV];
+  };
+  auto fetch = [&](int t0, Rows& f) {
     const long low = rev ? len - t0 - C : t0;  // (below zero only where the lanes of those rows do not load)
     const char* const ka = kbase + low * R.k.ld * (long)sizeof(T);
     const char* const va = vbase + low * R.v.ld * (long)sizeof(T);
     const char* const qa = OUT ? qbase + low * R.q.ld * (long)sizeof(T) : nullptr;
-    const int n_rows = end - t0;
-    if (n_rows >= C) {
+    const int rows = min(end - t0, C);  // (a thread without a piece of its own has a row behind the chunk)
+    if (rows == C && PIECES_K % THREADS == 0 && PIECES_V % THREADS == 0) {
 #pragma unroll
-      for (int n = 0; n < G::NK; ++n) {
-        kf[n] = *reinterpret_cast<const dec_u4*>(ka + koff[n]);
-        if (OUT) qf[n] = *reinterpret_cast<const dec_u4*>(qa + qoff[n]);
+      for (int n = 0; n < NK; ++n) {
+        f.k[n] = *reinterpret_cast<const dec_u4*>(ka + koff[n]);
+        if (OUT) f.q[n] = *reinterpret_cast<const dec_u4*>(qa + qoff[n]);
       }
 #pragma unroll
-      for (int n = 0; n < G::NV; ++n) vf[n] = *reinterpret_cast<const dec_u4*>(va + voff[n]);
+      for (int n = 0; n < NV; ++n) f.v[n] = *reinterpret_cast<const dec_u4*>(va + voff[n]);
     } else {
 #pragma unroll
-      for (int n = 0; n < G::NK; ++n) {
-        const bool in = (tid + n * G::THREADS) / (DK / VEC) < n_rows;
-        kf[n] = dec_u4(0u);
-        if (in) kf[n] = *reinterpret_cast<const dec_u4*>(ka + koff[n]);
+      for (int n = 0; n < NK; ++n) {
+        const bool in = krow(n) < rows;
+        f.k[n] = dec_u4(0u);
+        if (in) f.k[n] = *reinterpret_cast<const dec_u4*>(ka + koff[n]);
         if (OUT) {
-          qf[n] = dec_u4(0u);
-          if (in) qf[n] = *reinterpret_cast<const dec_u4*>(qa + qoff[n]);
+          f.q[n] = dec_u4(0u);
+          if (in) f.q[n] = *reinterpret_cast<const dec_u4*>(qa + qoff[n]);
         }
       }
 #pragma unroll
-      for (int n = 0; n < G::NV; ++n) {
-        vf[n] = dec_u4(0u);
-        if ((tid + n * G::THREADS) / (DV / VEC) < n_rows) vf[n] = *reinterpret_cast<const dec_u4*>(va + voff[n]);
+      for (int n = 0; n < NV; ++n) {
+        f.v[n] = dec_u4(0u);
+        if (vrow(n) < rows) f.v[n] = *reinterpret_cast<const dec_u4*>(va + voff[n]);
       }
     }
   };
-  auto stage = [&]() {
+  auto stage = [&](const Rows& f) {
 #pragma unroll
-    for (int n = 0; n < G::NK; ++n) {
-      const int u = tid + n * G::THREADS, at = u / (DK / VEC) * PK + u % (DK / VEC) * VEC;
-      *reinterpret_cast<dec_u4*>(ktile + at) = kf[n];
-      if (OUT) *reinterpret_cast<dec_u4*>(qtile + at) = qf[n];
+    for (int n = 0; n < NK; ++n) {
+      if (PIECES_K % THREADS != 0 && krow(n) >= C) continue;
+      *reinterpret_cast<dec_u4*>(ktile.piece(krow(n), kpiece(n))) = f.k[n];
+      if (OUT) *reinterpret_cast<dec_u4*>(qtile.piece(krow(n), kpiece(n))) = f.q[n];
     }
 #pragma unroll
-    for (int n = 0; n < G::NV; ++n) {
-      const int u = tid + n * G::THREADS;
-      *reinterpret_cast<dec_u4*>(vtile + u / (DV / VEC) * PV + u % (DV / VEC) * VEC) = vf[n];
+    for (int n = 0; n < NV; ++n) {
+      if (PIECES_V % THREADS != 0 && vrow(n) >= C) continue;
+      *reinterpret_cast<dec_u4*>(vtile.piece(vrow(n), vpiece(n))) = f.v[n];
     }
   };
-  if (s0 < end) fetch(s0);
+  Rows rows;  // one chunk ahead (two ahead measured the same, in twice the registers)
+  if (s0 < end) fetch(s0, rows);
 
-  // ---- powers of the decay: lambda^(i-j) is, tile by tile, the one of the places inside the tiles times a uniform one
   const float a2 = dec_log2(args.log_decay[h]);
   auto upow = [&](int n) { return dec_uniform(dec_pow(a2, n)); };
-  float wdiag[4], woff[4], wend[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int d = l16 - (4 * g + r);
-    wdiag[r] = dec_pow(a2, max(d, 0));
-    woff[r] = dec_pow(a2, 16 + d);
-    wend[r] = dec_pow(a2, 15 - (4 * g + r));
-  }
-  const float fq = dec_pow(a2, 16 * it + l16 + 1);
-
-  // ---- the state this segment starts from: tile (t, m), this lane: column scol + 16 m + l16, rows srow + 16 t + 4 g + r
-  dec_f4 S[KT][MS];
-#pragma unroll
-  for (int t = 0; t < KT; ++t)
-#pragma unroll
-    for (int m = 0; m < MS; ++m) S[t][m] = dec_f4(0.f);
-  const int splace = (srow + 4 * g) * DV + scol + l16;
-  const int wplace = wave * (KT * MS * 64) + lane;  // in the workspace the accumulators lie as they are
-  if (first && args.state) {
-    // (with several segments the copy is read, see above)
-    const float* sp = (OUT && !single ? R.ws + ((long)bh * args.segments + args.segments - 1) * (DK * DV)
-                                      : args.state + (long)bh * DK * DV) + splace;
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int m = 0; m < MS; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[t][m][r] = sp[(16 * t + r) * DV + 16 * m];
-  }
-  if (OUT && !first && s0 < len) {
-    // joined from the states at the ends of the earlier segments: sum over s' < seg of lambda^((seg-1-s') seg_len) E_s'
-    float w = 1.f;
-    const float lamL = upow(args.seg_len);
-    for (int s = seg - 1; s >= 0 && w != 0.f; --s, w *= lamL) {
-      const dec_f4* e = reinterpret_cast<const dec_f4*>(R.ws + ((long)bh * args.segments + s) * (DK * DV)) + wplace;
-#pragma unroll
-      for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int m = 0; m < MS; ++m) S[t][m] += w * e[(t * MS + m) * 64];
-    }
-  }
-
-  T* const op = (T*)R.out.p + (long)b * R.out.bs + (long)h * DV + 8 * g;
-  for (int t0 = s0; t0 < end; t0 += C) {
-    const int n = min(C, end - t0);  // frames of this chunk
-    __syncthreads();                 // everybody has finished with the previous one
-    stage();
-    if (OUT) {
-#pragma unroll
-      for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int m = 0; m < MS; ++m) dec_store4(stile + (scol + 16 * m + l16) * PK + srow + 16 * t + 4 * g, S[t][m]);
-    }
+  // A chunk's tiles: staged once everybody has finished with the previous ones, `hand_over` by the waves of the state.  The two
+  // kinds of waves run loops of their own (each keeps its own values in registers) that meet at the same barriers.
+  auto begin = [&](int t0, auto hand_over) {
     __syncthreads();
-    if (t0 + C < end) fetch(t0 + C);
+    stage(rows);
+    hand_over();
+    __syncthreads();
+    if (t0 + C < end) fetch(t0 + C, rows);
+  };
 
-    if (OUT && 16 * it < n) {
+  if (!holds) {
+    float wdiag[4], woff[4];  // lambda^(i-j) inside a tile, and 16 more: tile by tile times a uniform power
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = l16 - (4 * g + r);
+      wdiag[r] = dec_pow(a2, max(d, 0));
+      woff[r] = dec_pow(a2, 16 + d);
+    }
+    const float fq = dec_pow(a2, 16 * it + l16 + 1);
+    T* const op = (T*)R.out.p + (long)b * R.out.bs + (long)h * DV + 16 * mo0 + 4 * g;
+    for (int t0 = s0; t0 < end; t0 += C) {
+      begin(t0, [] {});
+      if (t0 + 16 * it >= end) continue;
       Frag qx[KB];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) dec_lds_frag(qx[kb], qtile + (16 * it + l16) * PK + kb * 32 + g * 8);
+      for (int kb = 0; kb < KB; ++kb) qx[kb] = qtile.row_frag(16 * it + l16, kb, g);
       dec_f4 o[MO];
 #pragma unroll
-      for (int i = 0; i < MO; ++i) {  // column tile mo: columns 32 (mo / 2) + 4 (mo % 2) + 8 (row / 4) + row % 4
-        const int mo = mo0 + i;
-        const T* const sr = stile + (32 * (mo >> 1) + 4 * (mo & 1) + 8 * (l16 >> 2) + (l16 & 3)) * PK + g * 8;
+      for (int i = 0; i < MO; ++i) {
         o[i] = dec_f4(0.f);
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          Frag sx;
-          dec_lds_frag(sx, sr + kb * 32);
-          o[i] = dec_mma(sx, qx[kb], o[i]);
-        }
+        for (int kb = 0; kb < KB; ++kb) o[i] = dec_mma(stile.row_frag(16 * (mo0 + i) + l16, kb, g), qx[kb], o[i]);
         o[i] *= fq;
       }
 #pragma unroll 1
@@ -396,11 +370,7 @@ __global__ __launch_bounds__(256, (DecGeo<T, DK, DV>::WAVES)) void k_decay(Decay
           p[x] = dec_f4(0.f);
           if (jt > it) continue;
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) {
-            Frag kx;
-            dec_lds_frag(kx, ktile + (16 * jt + l16) * PK + kb * 32 + g * 8);
-            p[x] = dec_mma(kx, qx[kb], p[x]);
-          }
+          for (int kb = 0; kb < KB; ++kb) p[x] = dec_mma(ktile.row_frag(16 * jt + l16, kb, g), qx[kb], p[x]);
           if (jt == it) {  // masked by selection: a frame behind this one contributes nothing, whatever it holds
 #pragma unroll
             for (int r = 0; r < 4; ++r) p[x][r] = l16 >= 4 * g + r ? p[x][r] * wdiag[r] : 0.f;
@@ -413,90 +383,128 @@ __global__ __launch_bounds__(256, (DecGeo<T, DK, DV>::WAVES)) void k_decay(Decay
         Frag pf;
         dec_pack(pf, p[0], p[1]);
 #pragma unroll
-        for (int i = 0; i < MO; ++i) {
-          const int mo = mo0 + i;
-          Frag vx;
-          dec_cols_spread<PV>(vx, vtile + jb * 32 * PV + 32 * (mo >> 1) + 4 * (mo & 1), l16, g);
-          o[i] = dec_mma(vx, pf, o[i]);
-        }
+        for (int i = 0; i < MO; ++i) o[i] = dec_mma(vtile.col_frag(32 * jb, 16 * (mo0 + i), l16, g), pf, o[i]);
       }
       const int t = t0 + 16 * it + l16;
       if (t < end) {
         T* const dst = op + (long)(rev ? len - 1 - t : t) * R.out.ld;
-        if constexpr (MO == 1) {
-          dec_store4(dst + 32 * (mo0 >> 1) + 4 * (mo0 & 1), o[0] * args.scale);
-        } else {
 #pragma unroll
-          for (int i = 0; i < MO; i += 2) dec_store8(dst + 16 * (mo0 + i), o[i] * args.scale, o[i + 1] * args.scale);
-        }
+        for (int i = 0; i < MO; ++i) dec_store4(dst + 16 * i, o[i] * args.scale);
       }
     }
-
-    // ---- the state behind the chunk
-    const float lam = upow(n);
+  } else {
+    // ---- the state this segment starts from: tile (t, m), this lane: column scol + 16 m + l16, rows srow + 16 t + 4 g + r
+    dec_f4 S[KT][MS];
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int m = 0; m < MS; ++m) S[t][m] *= lam;
+      for (int m = 0; m < MS; ++m) S[t][m] = dec_f4(0.f);
+    const int splace = (srow + 4 * g) * DV + scol + l16;
+    const int wplace = wave * (KT * MS * 64) + lane;  // in the workspace the accumulators lie as they are
+    if (first && args.state) {
+      // (with several segments the copy is read, see above)
+      const float* sp = (OUT && !single ? R.ws + ((long)bh * args.segments + args.segments - 1) * (DK * DV)
+                                        : args.state + (long)bh * DK * DV) + splace;
 #pragma unroll
-    for (int jb = 0; jb < JB; ++jb) {
-      float w[8];  // lambda^(n-1-j) of this lane's frames (those behind the end hold zeros)
-      if (n == C) {
-        const float w0 = upow(C - 16 - 32 * jb), w1 = upow(C - 32 - 32 * jb);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = wend[e] * w0, w[4 + e] = wend[e] * w1;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = dec_pow(a2, max(n - 1 - (jb * 32 + (e >> 2) * 16 + 4 * g + (e & 3)), 0));
-      }
-      Frag wv[MS][sizeof(T) == 2 ? TERMS : 1];
-#pragma unroll
-      for (int m = 0; m < MS; ++m) {
-        Frag vx;
-        dec_cols<PV>(vx, vtile + jb * 32 * PV + scol + 16 * m, l16, g);
-        if constexpr (sizeof(T) == 2) {
-          dec_split<TERMS>(vx, w, wv[m]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) wv[m][0].a[e] = vx.a[e] * w[e], wv[m][0].b[e] = vx.b[e] * w[4 + e];
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        Frag kx;
-        dec_cols<PK>(kx, ktile + jb * 32 * PK + srow + 16 * t, l16, g);
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int m = 0; m < MS; ++m)
 #pragma unroll
-          for (int x = (sizeof(T) == 2 ? TERMS : 1) - 1; x >= 0; --x) S[t][m] = dec_mma(kx, wv[m][x], S[t][m]);
+          for (int r = 0; r < 4; ++r) S[t][m][r] = sp[(16 * t + r) * DV + 16 * m];
+    }
+    if (OUT && !first && s0 < len) {
+      // sum over s' < seg of lambda^((seg-1-s') seg_len) E_s' of the states E at the ends of the segments before; where there
+      // are many, k_decay_join has summed them
+      const float lamL = upow(args.seg_len);
+      float w = 1.f;
+      const int from = args.joined ? seg - 1 : 0;
+      for (int s = seg - 1; s >= from; --s, w *= lamL) {
+        const dec_f4* e = reinterpret_cast<const dec_f4*>(R.ws + ((long)bh * args.segments + s) * (DK * DV)) + wplace;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int m = 0; m < MS; ++m) S[t][m] += w * e[(t * MS + m) * 64];
       }
     }
-  }
 
-  if (!OUT) {
-    dec_f4* e = reinterpret_cast<dec_f4*>(R.ws + ((long)bh * args.segments + seg) * (DK * DV)) + wplace;
+    float wend[4];  // lambda^(15-j) inside a tile
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
+    for (int r = 0; r < 4; ++r) wend[r] = dec_pow(a2, 15 - (4 * g + r));
+    for (int t0 = s0; t0 < end; t0 += C) {
+      const int n = min(C, end - t0);  // frames of this chunk
+      begin(t0, [&] {
+        if (OUT) {
 #pragma unroll
-      for (int m = 0; m < MS; ++m) e[(t * MS + m) * 64] = S[t][m];
-    return;
+          for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int m = 0; m < MS; ++m) stile.put4(scol + 16 * m + l16, srow + 16 * t + 4 * g, S[t][m]);
+        }
+      });
+      const float lam = upow(n);
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int m = 0; m < MS; ++m) S[t][m] *= lam;
+#pragma unroll
+      for (int jb = 0; jb < JB; ++jb) {
+        float w[8];  // lambda^(n-1-j) of this lane's frames (those behind the end hold zeros)
+        if (n == C) {
+          const float w0 = upow(C - 16 - 32 * jb), w1 = upow(C - 32 - 32 * jb);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = wend[e] * w0, w[4 + e] = wend[e] * w1;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = dec_pow(a2, max(n - 1 - (jb * 32 + (e >> 2) * 16 + 4 * g + (e & 3)), 0));
+        }
+        Frag wv[MS][sizeof(T) == 2 ? TERMS : 1];
+#pragma unroll
+        for (int m = 0; m < MS; ++m) {
+          const Frag vx = vtile.col_frag(32 * jb, scol + 16 * m, l16, g);
+          if constexpr (sizeof(T) == 2) {
+            dec_split<TERMS>(vx, w, wv[m]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) wv[m][0].a[e] = vx.a[e] * w[e], wv[m][0].b[e] = vx.b[e] * w[4 + e];
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          const Frag kx = ktile.col_frag(32 * jb, srow + 16 * t, l16, g);
+#pragma unroll
+          for (int m = 0; m < MS; ++m)
+#pragma unroll
+            for (int x = (sizeof(T) == 2 ? TERMS : 1) - 1; x >= 0; --x) S[t][m] = dec_mma(kx, wv[m][x], S[t][m]);
+        }
+      }
+    }
+
+    if (!OUT) {
+      dec_f4* e = reinterpret_cast<dec_f4*>(R.ws + ((long)bh * args.segments + seg) * (DK * DV)) + wplace;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int m = 0; m < MS; ++m) e[(t * MS + m) * 64] = S[t][m];
+    } else if (args.state && s0 < len && s1 >= len) {
+      // the final state, by the segment that holds the last frame (an empty utterance keeps what it had)
+      float* sp = args.state + (long)bh * DK * DV + splace;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int m = 0; m < MS; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sp[(16 * t + r) * DV + 16 * m] = S[t][m][r];
+    }
   }
+  if (!OUT) return;
   // zeros behind the utterance's end
-  for (int i = max(s0, len) * (DV / VEC) + tid; i < s1 * (DV / VEC); i += G::THREADS) {
+  for (int i = max(s0, len) * (DV / VEC) + tid; i < s1 * (DV / VEC); i += THREADS) {
     const int t = i / (DV / VEC), c = (i % (DV / VEC)) * VEC;
     *reinterpret_cast<dec_u4*>((T*)R.out.p + (long)b * R.out.bs + (long)t * R.out.ld + (long)h * DV + c) = dec_u4(0u);
   }
-  // the final state, by the segment that holds the last frame (an empty utterance keeps what it had)
-  if (args.state && s0 < len && s1 >= len) {
-    float* sp = args.state + (long)bh * DK * DV + splace;
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int m = 0; m < MS; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sp[(16 * t + r) * DV + 16 * m] = S[t][m][r];
-  }
 }
+
+// The states at the ends of the segments (decay.hip): E_s becomes sum over s' <= s of lambda^((s-s') seg_len) E_s'.
+int decay_launch_join(const DecayArgs& a, int roles, int state_elements, hipStream_t st);
 
 template <class T, int DK, int DV, int TERMS>
 static int decay_launch_terms(const DecayArgs& a, int roles, hipStream_t st) {
@@ -509,12 +517,13 @@ static int decay_launch_terms(const DecayArgs& a, int roles, hipStream_t st) {
   }
   if (a.segments > 1) {
     ProfScope ps("k_decay_states", st);
-    hipLaunchKernelGGL((k_decay<T, DK, DV, false, TERMS>), dim3(a.B * a.H, a.segments - 1, roles), dim3(G::THREADS),
+    hipLaunchKernelGGL((k_decay<T, DK, DV, false, TERMS>), dim3(a.B * a.H, a.segments - 1, roles), dim3(256),
                        G::kLdsState, st, a);
+    if (a.joined && decay_launch_join(a, roles, DK * DV, st)) return 1;
   }
   {
     ProfScope ps("k_decay", st);
-    hipLaunchKernelGGL((k_decay<T, DK, DV, true, TERMS>), dim3(a.B * a.H, a.segments, roles), dim3(G::THREADS), G::kLdsOut,
+    hipLaunchKernelGGL((k_decay<T, DK, DV, true, TERMS>), dim3(a.B * a.H, a.segments, roles), dim3(512), G::kLdsOut,
                        st, a);
   }
   const hipError_t e = hipGetLastError();

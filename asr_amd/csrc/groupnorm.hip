@@ -10,15 +10,15 @@
 //
 // A thread owns V neighbouring channels of one group (V = what divides C / G, up to 16 bytes), so every load is as wide as
 // the group allows and one partial sum serves the V values.
-//   rows (T = 1, no lengths): a row's C / V threads hold it in registers -- one read, one write -- and sum a group over its threads by
-//     shuffles when they are a power of two, through LDS otherwise.
+//   rows (T = 1, no lengths): a row's C / V threads hold it in registers -- one read, one write -- and sum a group over its
+//     threads by shuffles when they are a power of two, through LDS otherwise.
 //   utterances, columns: where an utterance's frames of a few groups fit a workgroup's registers, it reads them once, keeps
 //     them, and writes the result: one launch, one read, one write.
 //   utterances, splits: otherwise the frames are split over workgroups.  k_gn_stats leaves (count, mean, centred second
 //     moment) of each split and group, k_gn_apply joins them and normalises, reading x again.  The backward does the same
 //     with the per-channel sums of dz and dz xhat, from which the group sums and the parameter gradients both follow.
-// Sums are 32-bit, second moments about a value of the data, never as a difference of large sums; the moments of
-// different threads are joined in 64 bits.  Fixed order, no atomics.  HBM-bound.
+// Second moments are taken about a value of the data, never as a difference of large sums.  The utterances' statistics are
+// summed in 64 bits, everything else in 32.  Fixed order, no atomics.  HBM-bound.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -44,11 +44,23 @@ __device__ __forceinline__ float gn_act(float z, int act) {
   if (act == kGnSilu) return z * gn_sigmoid(z);
   return z;
 }
-__device__ __forceinline__ float gn_slope(float z, int act) {
-  if (act == kGnRelu) return z > 0.f ? 1.f : 0.f;
+// A group's statistics as the element-wise arithmetic takes them, and in 64 bits.
+struct GnStat {
+  float mean, rstd;
+  double dmean, drstd;
+};
+__device__ __forceinline__ GnStat gn_stat(const double2& s) { return GnStat{(float)s.x, (float)s.y, s.x, s.y}; }
+// act'(z) at z = (x - mean) rstd w + b.  The ReLU's slope jumps at zero, and one element on the wrong side is a whole dy in dx
+// and in the sums: a z within the 32-bit arithmetic's error of zero is decided in 64 bits (a few in a million).
+__device__ __forceinline__ float gn_slope(float z, float x, float w, float b, const GnStat& s, int act) {
+  if (act == kGnRelu) {
+    if (fabsf(z) <= 5e-7f * (fabsf(b) + (fabsf(x) + fabsf(s.mean)) * fabsf(s.rstd * w)))
+      return ((double)x - s.dmean) * s.drstd * (double)w + (double)b > 0. ? 1.f : 0.f;
+    return z > 0.f ? 1.f : 0.f;
+  }
   if (act == kGnSilu) {
-    const float s = gn_sigmoid(z);
-    return s * (1.f + z * (1.f - s));
+    const float y = gn_sigmoid(z);
+    return y * (1.f + z * (1.f - y));
   }
   return 1.f;
 }
@@ -130,7 +142,7 @@ struct GnArgs {
   const float* beta;
   const int* lengths;  // [N] or NULL
   void* out;           // y, or dx
-  float* stats;        // [N][G][2]: mean, rstd
+  double2* stats;      // [N][G]: mean, rstd
   float* part;         // workspace
   float eps;
   long N;
@@ -138,10 +150,10 @@ struct GnArgs {
 };
 
 // sum over the L neighbouring threads of a group (this thread's first one is g0; `groups` in the workgroup).  POW2: by
-// shuffles.  Otherwise through red (one float a thread, one a group behind them): few threads a group are summed by each of
+// shuffles.  Otherwise through red (one value a thread, one a group behind them): few threads a group are summed by each of
 // them, many by a team of lanes (125 threads a group, 3000 x 1000 in 8 groups: 50 us if each thread sums them all).
-template <bool POW2>
-__device__ __forceinline__ float gn_group_sum(float v, int L, int g0, int groups, float* red) {
+template <bool POW2, class F>
+__device__ __forceinline__ F gn_group_sum(F v, int L, int g0, int groups, F* red) {
   if (POW2) {
     for (int o = L >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
     return v;
@@ -149,7 +161,7 @@ __device__ __forceinline__ float gn_group_sum(float v, int L, int g0, int groups
   __syncthreads();
   red[threadIdx.x] = v;
   __syncthreads();
-  float s = 0.f;
+  F s = 0;
   if (L <= 16) {
     for (int i = 0; i < L; ++i) s += red[g0 + i];
     return s;
@@ -157,7 +169,7 @@ __device__ __forceinline__ float gn_group_sum(float v, int L, int g0, int groups
   const int lanes = L <= 128 ? 16 : 64, lane = threadIdx.x & (lanes - 1);
   for (int t0 = 0; t0 < groups; t0 += blockDim.x / lanes) {  // uniform: the shuffles need every lane
     const int t = t0 + threadIdx.x / lanes;
-    s = 0.f;
+    s = 0;
     if (t < groups)
       for (int i = lane; i < L; i += lanes) s += red[t * L + i];
     for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
@@ -244,7 +256,8 @@ __global__ __launch_bounds__(1024) void k_gn_rows(GnArgs a) {
 // the workgroup leaves one partial [2][C] (dgamma, dbeta) in part[blockIdx].
 template <bool XB, bool GB, int V, bool POW2>
 __global__ __launch_bounds__(1024) void k_gn_rows_bwd(GnArgs a) {
-  __shared__ float red[POW2 ? 1 : 1024 + 1024];
+  __shared__ double dred[POW2 ? 1 : 1024 + 1024];
+  float* const red = reinterpret_cast<float*>(dred);
   extern __shared__ float gn_sums[];
   const int TR = a.C / V, RB = blockDim.x / TR, cg = a.C / a.G, L = cg / V;
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V, g0 = threadIdx.x - (threadIdx.x % TR) % L;
@@ -261,34 +274,45 @@ __global__ __launch_bounds__(1024) void k_gn_rows_bwd(GnArgs a) {
     const long row = r0 + slot;
     const bool live = on && row < a.N;
     GnVec<V> x, dy;
-    float s = 0.f;
 #pragma unroll
     for (int e = 0; e < V; ++e) x.f[e] = dy.f[e] = 0.f;
     if (live) {
       x = gn_load<XB, V>(a.x, row * a.C + c);
       dy = gn_load<GB, V>(a.dy, row * a.C + c);
+    }
+    GnStat st;
+    if (a.act == kGnRelu) {  // (whose slope asks for them in 64 bits)
+      double s = 0.;
 #pragma unroll
       for (int e = 0; e < V; ++e) s += x.f[e];
-    }
-    const float mean = gn_group_sum<POW2>(s, L, g0, RB * a.G, red) * inv_n;
-    s = 0.f;
+      const double mean = gn_group_sum<POW2>(s, L, g0, RB * a.G, dred) / cg;
+      s = 0.;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      x.f[e] -= mean;
-      s += x.f[e] * x.f[e];
+      for (int e = 0; e < V; ++e) s += (x.f[e] - mean) * (x.f[e] - mean);
+      st = gn_stat(make_double2(mean, 1. / sqrt(gn_group_sum<POW2>(s, L, g0, RB * a.G, dred) / cg + (double)a.eps)));
+    } else {
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += x.f[e];
+      st.mean = gn_group_sum<POW2>(s, L, g0, RB * a.G, red) * inv_n;
+      s = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += (x.f[e] - st.mean) * (x.f[e] - st.mean);
+      st.rstd = rsqrtf(gn_group_sum<POW2>(s, L, g0, RB * a.G, red) * inv_n + a.eps);
     }
-    const float rstd = rsqrtf(gn_group_sum<POW2>(s, L, g0, RB * a.G, red) * inv_n + a.eps);
+    const float rstd = st.rstd;
     float s1 = 0.f, s2 = 0.f;
     if (live) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        x.f[e] *= rstd;  // xhat
-        const float dz = dy.f[e] * gn_slope(x.f[e] * g.f[e] + bt.f[e], a.act);
+        const float h = (x.f[e] - st.mean) * rstd;  // xhat
+        const float dz = dy.f[e] * gn_slope(h * g.f[e] + bt.f[e], x.f[e], g.f[e], bt.f[e], st, a.act);
+        x.f[e] = h;
         db.f[e] += dz;
-        dg.f[e] += dz * x.f[e];
+        dg.f[e] += dz * h;
         dy.f[e] = dz * g.f[e];
         s1 += dy.f[e];
-        s2 += dy.f[e] * x.f[e];
+        s2 += dy.f[e] * h;
       }
     }
     s1 = gn_group_sum<POW2>(s1, L, g0, RB * a.G, red) * inv_n;
@@ -318,13 +342,24 @@ __device__ __forceinline__ GnMoment gn_join(const GnMoment& p, const GnMoment& q
 __device__ __forceinline__ int gn_len(const GnArgs& a, long n) { return a.lengths ? min(max(a.lengths[n], 0), a.T) : a.T; }
 
 // The moments of cnt values from the sum and the sum of squares of their distances from a pivot.
-__device__ __forceinline__ GnMoment gn_moment(double cnt, float pivot, float s, float ss) {
+__device__ __forceinline__ GnMoment gn_moment(double cnt, float pivot, double s, double ss) {
   if (cnt <= 0.) return GnMoment{0., 0., 0.};
-  const double m2 = (double)ss - (double)s * s / cnt;
-  return GnMoment{cnt, pivot + (double)s / cnt, m2 < 0. ? 0. : m2};
+  const double m2 = ss - s * s / cnt;
+  return GnMoment{cnt, pivot + s / cnt, m2 < 0. ? 0. : m2};
 }
-__device__ __forceinline__ float2 gn_mean_rstd(const GnMoment& t, float eps) {
-  return make_float2((float)t.mean, (float)(1. / sqrt((t.n > 0. ? t.m2 / t.n : 0.) + (double)eps)));
+__device__ __forceinline__ double2 gn_mean_rstd(const GnMoment& t, float eps) {
+  return make_double2(t.mean, 1. / sqrt((t.n > 0. ? t.m2 / t.n : 0.) + (double)eps));
+}
+// A vector's part of the sums about the pivot, in 64 bits: memory is waited for anyway, and the ReLU's border asks for a mean
+// that is exact (gn_slope).
+template <int V>
+__device__ __forceinline__ void gn_add_moments(const GnVec<V>& x, double pivot, double& s, double& ss) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const double d = (double)x.f[e] - pivot;
+    s += d;
+    ss = fma(d, d, ss);
+  }
 }
 // frames first..last-1 of this thread's channels: zeros
 template <bool OB, int V>
@@ -336,13 +371,13 @@ __device__ __forceinline__ void gn_zero_frames(const GnArgs& a, long base, int f
 }
 template <int V>
 __device__ __forceinline__ GnVec<V> gn_dx(const GnVec<V>& x, const GnVec<V>& dy, const GnVec<V>& g, const GnVec<V>& bt,
-                                          const float2& ms, const float2& m, int act) {
+                                          const GnStat& st, const float2& m, int act) {
   GnVec<V> d;
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const float h = (x.f[e] - ms.x) * ms.y;
-    const float dz = dy.f[e] * gn_slope(h * g.f[e] + bt.f[e], act);
-    d.f[e] = (dz * g.f[e] - m.x - h * m.y) * ms.y;
+    const float h = (x.f[e] - st.mean) * st.rstd;
+    const float dz = dy.f[e] * gn_slope(h * g.f[e] + bt.f[e], x.f[e], g.f[e], bt.f[e], st, act);
+    d.f[e] = (dz * g.f[e] - m.x - h * m.y) * st.rstd;
   }
   return d;
 }
@@ -350,11 +385,11 @@ __device__ __forceinline__ GnVec<V> gn_dx(const GnVec<V>& x, const GnVec<V>& dy,
 // ---- utterances.  Threads of a row own V channels each, the workgroup's rows of threads take its frames in turn.
 //
 // Sums of a group: (sum, sum of squares) of x - pivot over the threads of the group, the pivot being one value of the group
-// that all its threads take, so the partials of a workgroup simply add up.  red: one float2 a thread.  The threads
+// that all its threads take, so the partials of a workgroup simply add up.  red: one double2 a thread.  The threads
 // tid / lanes, each team of `lanes` (a power of two up to 64) joining one group at a time, call `put(group, sum, squares)`.
 template <class F>
-__device__ __forceinline__ void gn_join_groups(float s, float ss, int TR, int RB, int L, int G, float2* red, F put) {
-  red[threadIdx.x] = make_float2(s, ss);
+__device__ __forceinline__ void gn_join_groups(double s, double ss, int TR, int RB, int L, int G, double2* red, F put) {
+  red[threadIdx.x] = make_double2(s, ss);
   __syncthreads();
   const int parts = RB * L;
   int lanes = 1;
@@ -362,10 +397,10 @@ __device__ __forceinline__ void gn_join_groups(float s, float ss, int TR, int RB
   const int team = threadIdx.x / lanes, lane = threadIdx.x % lanes;
   for (int g0 = 0; g0 < G; g0 += blockDim.x / lanes) {  // uniform: the shuffles need every lane
     const int g = g0 + team;
-    float a = 0.f, b = 0.f;
+    double a = 0., b = 0.;
     if (g < G)
       for (int i = lane; i < parts; i += lanes) {
-        const float2 p = red[(i / L) * TR + g * L + i % L];
+        const double2 p = red[(i / L) * TR + g * L + i % L];
         a += p.x;
         b += p.y;
       }
@@ -380,28 +415,23 @@ __device__ __forceinline__ void gn_join_groups(float s, float ss, int TR, int RB
 // Workgroup (split, n) of the statistics over several workgroups: each split's moments of each group.
 template <bool XB, int V>
 __global__ __launch_bounds__(1024) void k_gn_stats(GnArgs a) {
-  __shared__ float2 red[1024];
+  __shared__ double2 red[1024];
   const int TR = a.C / V, RB = blockDim.x / TR, cg = a.C / a.G, L = cg / V;
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V;
   const long n = blockIdx.y;
   const int t0 = blockIdx.x * a.split_len, t1 = min(t0 + a.split_len, gn_len(a, n));
   const long base = n * a.T * a.C;
-  float s = 0.f, ss = 0.f;
+  double s = 0., ss = 0.;
   if (slot < RB && t0 < t1) {
     const float pivot = gn_load<XB, 1>(a.x, base + (long)t0 * a.C + c / cg * cg).f[0];
 #pragma unroll 4
     for (int t = t0 + slot; t < t1; t += RB) {
       const GnVec<V> x = gn_load<XB, V>(a.x, base + (long)t * a.C + c);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float d = x.f[e] - pivot;
-        s += d;
-        ss += d * d;
-      }
+      gn_add_moments<V>(x, pivot, s, ss);
     }
   }
   GnMoment* const out = reinterpret_cast<GnMoment*>(a.part) + (n * a.splits + blockIdx.x) * a.G;
-  gn_join_groups(s, ss, TR, RB, L, a.G, red, [&](int g, float u, float v) {
+  gn_join_groups(s, ss, TR, RB, L, a.G, red, [&](int g, double u, double v) {
     const double cnt = (double)max(t1 - t0, 0) * cg;
     const float pivot = cnt > 0. ? gn_load<XB, 1>(a.x, base + (long)t0 * a.C + g * cg).f[0] : 0.f;
     out[g] = gn_moment(cnt, pivot, u, v);
@@ -410,7 +440,7 @@ __global__ __launch_bounds__(1024) void k_gn_stats(GnArgs a) {
 
 template <bool XB, bool OB, int V>
 __global__ __launch_bounds__(1024) void k_gn_apply(GnArgs a) {
-  __shared__ float2 st[kGnMaxWidth];  // [G]
+  __shared__ double2 st[kGnMaxWidth];  // [G]
   const int TR = a.C / V, RB = blockDim.x / TR, cg = a.C / a.G;
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V;
   const long n = blockIdx.y;
@@ -418,19 +448,19 @@ __global__ __launch_bounds__(1024) void k_gn_apply(GnArgs a) {
     GnMoment t{0., 0., 0.};
     for (int s = 0; s < a.splits; ++s) t = gn_join(t, *(reinterpret_cast<const GnMoment*>(a.part) + (n * a.splits + s) * a.G + g));
     st[g] = gn_mean_rstd(t, a.eps);
-    if (a.stats && blockIdx.x == 0) *reinterpret_cast<float2*>(a.stats + (n * a.G + g) * 2) = st[g];
+    if (a.stats && blockIdx.x == 0) a.stats[n * a.G + g] = st[g];
   }
   __syncthreads();
   if (slot >= RB) return;
   const GnVec<V> g = gn_load<false, V>(a.gamma, c), bt = gn_load<false, V>(a.beta, c);
-  const float2 ms = st[c / cg];
+  const GnStat st_ = gn_stat(st[c / cg]);
   const int len = gn_len(a, n), t0 = blockIdx.x * a.split_len, t1 = min(t0 + a.split_len, a.T);
   const long base = n * a.T * a.C + c;
 #pragma unroll 4
   for (int t = t0 + slot; t < min(t1, len); t += RB) {
     GnVec<V> y = gn_load<XB, V>(a.x, base + (long)t * a.C);
 #pragma unroll
-    for (int e = 0; e < V; ++e) y.f[e] = gn_act((y.f[e] - ms.x) * ms.y * g.f[e] + bt.f[e], a.act);
+    for (int e = 0; e < V; ++e) y.f[e] = gn_act((y.f[e] - st_.mean) * st_.rstd * g.f[e] + bt.f[e], a.act);
     gn_store<OB, V>(a.out, base + (long)t * a.C, y);
   }
   gn_zero_frames<OB, V>(a, base, max(t0, len), t1, slot, RB);
@@ -451,14 +481,14 @@ __global__ __launch_bounds__(1024) void k_gn_bwd_sums(GnArgs a) {
   for (int e = 0; e < V; ++e) dg.f[e] = db.f[e] = 0.f;
   if (on) {
     const GnVec<V> g = gn_load<false, V>(a.gamma, c), bt = gn_load<false, V>(a.beta, c);
-    const float2 ms = *reinterpret_cast<const float2*>(a.stats + (n * a.G + c / cg) * 2);
+    const GnStat st = gn_stat(a.stats[n * a.G + c / cg]);
 #pragma unroll 4
     for (int t = t0 + slot; t < t1; t += RB) {
       const GnVec<V> x = gn_load<XB, V>(a.x, base + (long)t * a.C), dy = gn_load<GB, V>(a.dy, base + (long)t * a.C);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float h = (x.f[e] - ms.x) * ms.y;
-        const float dz = dy.f[e] * gn_slope(h * g.f[e] + bt.f[e], a.act);
+        const float h = (x.f[e] - st.mean) * st.rstd;
+        const float dz = dy.f[e] * gn_slope(h * g.f[e] + bt.f[e], x.f[e], g.f[e], bt.f[e], st, a.act);
         db.f[e] += dz;
         dg.f[e] += dz * h;
       }
@@ -502,14 +532,14 @@ __global__ __launch_bounds__(1024) void k_gn_bwd_apply(GnArgs a) {
   const int len = gn_len(a, n);
   if (slot >= RB) return;
   const GnVec<V> g = gn_load<false, V>(a.gamma, c), bt = gn_load<false, V>(a.beta, c);
-  const float2 ms = *reinterpret_cast<const float2*>(a.stats + (n * a.G + c / cg) * 2);
+  const GnStat st = gn_stat(a.stats[n * a.G + c / cg]);
   const float2 m = reinterpret_cast<const float2*>(a.part + a.N * a.splits * 2 * a.C)[n * a.G + c / cg];
   const int t0 = blockIdx.x * a.split_len, t1 = min(t0 + a.split_len, a.T);
   const long base = n * a.T * a.C + c;
 #pragma unroll 4
   for (int t = t0 + slot; t < min(t1, len); t += RB) {
     const GnVec<V> x = gn_load<XB, V>(a.x, base + (long)t * a.C), dy = gn_load<GB, V>(a.dy, base + (long)t * a.C);
-    gn_store<XB, V>(a.out, base + (long)t * a.C, gn_dx<V>(x, dy, g, bt, ms, m, a.act));
+    gn_store<XB, V>(a.out, base + (long)t * a.C, gn_dx<V>(x, dy, g, bt, st, m, a.act));
   }
   gn_zero_frames<XB, V>(a, base, max(t0, len), t1, slot, RB);
 }
@@ -529,8 +559,8 @@ __device__ __forceinline__ bool gn_column_place(const GnArgs& a, long* n, int* b
 
 template <bool XB, bool OB, int V, int NV>
 __global__ __launch_bounds__(1024) void k_gn_column(GnArgs a) {
-  __shared__ float2 red[1024];
-  __shared__ float2 st[1024];  // [groups of the block]: no more than its threads of a row
+  __shared__ double2 red[1024];
+  __shared__ double2 st[1024];  // [groups of the block]: no more than its threads of a row
   long n;
   int block;
   if (!gn_column_place(a, &n, &block)) return;
@@ -545,37 +575,31 @@ __global__ __launch_bounds__(1024) void k_gn_column(GnArgs a) {
     const int t = slot + i * RB;
     if (t < len) x[i].load(a.x, base + (long)t * a.C);
   }
-  float s = 0.f, ss = 0.f;
+  double s = 0., ss = 0.;
   const float pivot = len > 0 ? gn_load<XB, 1>(a.x, first + col / cg * cg).f[0] : 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     if (slot + i * RB < len) {
-      const GnVec<V> v = x[i].get();
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float d = v.f[e] - pivot;
-        s += d;
-        ss += d * d;
-      }
+      gn_add_moments<V>(x[i].get(), pivot, s, ss);
     }
   }
-  gn_join_groups(s, ss, TR, RB, L, groups, red, [&](int g, float u, float v) {
+  gn_join_groups(s, ss, TR, RB, L, groups, red, [&](int g, double u, double v) {
     const int frames = gn_len(a, n);
     const float p = frames > 0 ? gn_load<XB, 1>(a.x, first + g * cg).f[0] : 0.f;
     st[g] = gn_mean_rstd(gn_moment((double)frames * cg, p, u, v), a.eps);
-    if (a.stats) *reinterpret_cast<float2*>(a.stats + (n * a.G + block * groups + g) * 2) = st[g];
+    if (a.stats) a.stats[n * a.G + block * groups + g] = st[g];
   });
   __syncthreads();
   if (!on) return;
   const GnVec<V> g = gn_load<false, V>(a.gamma, c), bt = gn_load<false, V>(a.beta, c);
-  const float2 ms = st[col / cg];
+  const GnStat st_ = gn_stat(st[col / cg]);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int t = slot + i * RB;
     if (t < len) {
       GnVec<V> y = x[i].get();
 #pragma unroll
-      for (int e = 0; e < V; ++e) y.f[e] = gn_act((y.f[e] - ms.x) * ms.y * g.f[e] + bt.f[e], a.act);
+      for (int e = 0; e < V; ++e) y.f[e] = gn_act((y.f[e] - st_.mean) * st_.rstd * g.f[e] + bt.f[e], a.act);
       gn_store<OB, V>(a.out, base + (long)t * a.C, y);
     }
   }
@@ -614,19 +638,19 @@ __global__ __launch_bounds__(1024) void k_gn_column_bwd(GnArgs a) {
   GnVec<V> dg, db, g;
 #pragma unroll
   for (int e = 0; e < V; ++e) dg.f[e] = db.f[e] = 0.f;
-  float2 ms = make_float2(0.f, 0.f);
+  GnStat st{0.f, 0.f, 0., 0.};
   if (on) {
     g = gn_load<false, V>(a.gamma, c);
     const GnVec<V> bt = gn_load<false, V>(a.beta, c);
-    ms = *reinterpret_cast<const float2*>(a.stats + (n * a.G + c / cg) * 2);
+    st = gn_stat(a.stats[n * a.G + c / cg]);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (slot + i * RB < len) {
         const GnVec<V> xv = x[i].get();
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float h = (xv.f[e] - ms.x) * ms.y;
-          dz[i].f[e] *= gn_slope(h * g.f[e] + bt.f[e], a.act);
+          const float h = (xv.f[e] - st.mean) * st.rstd;
+          dz[i].f[e] *= gn_slope(h * g.f[e] + bt.f[e], xv.f[e], g.f[e], bt.f[e], st, a.act);
           db.f[e] += dz[i].f[e];
           dg.f[e] += dz[i].f[e] * h;
         }
@@ -654,7 +678,7 @@ __global__ __launch_bounds__(1024) void k_gn_column_bwd(GnArgs a) {
     if (t < len) {
       GnVec<V> d = x[i].get();
 #pragma unroll
-      for (int e = 0; e < V; ++e) d.f[e] = (dz[i].f[e] * g.f[e] - m.x - (d.f[e] - ms.x) * ms.y * m.y) * ms.y;
+      for (int e = 0; e < V; ++e) d.f[e] = (dz[i].f[e] * g.f[e] - m.x - (d.f[e] - st.mean) * st.rstd * m.y) * st.rstd;
       gn_store<XB, V>(a.out, base + (long)t * a.C, d);
     }
   }
@@ -810,14 +834,14 @@ extern "C" size_t lmufft_group_norm_workspace_bytes(int64_t N, int32_t T, int32_
 
 extern "C" int lmufft_group_norm(const void* x, int x_dtype, const float* gamma, const float* beta, const int32_t* lengths,
                                  int64_t N, int32_t T, int32_t C, int32_t G, float eps, int act, void* out, int out_dtype,
-                                 float* stats, void* workspace, size_t workspace_bytes, void* stream) {
+                                 double* stats, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "group norm";
   if (gn_check(what, x_dtype, out_dtype, N, T, C, G, act)) return 1;
   if (N == 0 || T == 0) return 0;
   if (!x || !gamma || !beta || !out) return set_error("%s: NULL pointer", what);
   const bool rows = T == 1 && !lengths;  // every row a sample of its own
   if (!rows && N > 65535) return set_error("%s: %lld utterances (at most 65535)", what, (long long)N);
-  if (!gn_aligned(x) || !gn_aligned(gamma) || !gn_aligned(beta) || !gn_aligned(out) || (reinterpret_cast<uintptr_t>(stats) & 7))
+  if (!gn_aligned(x) || !gn_aligned(gamma) || !gn_aligned(beta) || !gn_aligned(out) || !gn_aligned(stats))
     return set_error("%s: tensors must start on 16-byte boundaries", what);
   GnPlan p;
   const bool xb = x_dtype == LMUFFT_BF16, ob = out_dtype == LMUFFT_BF16;
@@ -825,7 +849,7 @@ extern "C" int lmufft_group_norm(const void* x, int x_dtype, const float* gamma,
   const size_t need = gn_workspace(p, N, C, G, false);
   if (need && (!workspace || workspace_bytes < need || !gn_aligned(workspace)))
     return set_error("%s: workspace of %zu bytes on a 16-byte boundary needed, %zu given", what, need, workspace_bytes);
-  GnArgs a{x, nullptr, gamma, beta, lengths, out, stats, (float*)workspace, eps, (long)N, T, C, G, act, p.splits, p.split_len};
+  GnArgs a{x, nullptr, gamma, beta, lengths, out, (double2*)stats, (float*)workspace, eps, (long)N, T, C, G, act, p.splits, p.split_len};
   hipStream_t st = (hipStream_t)stream;
   const dim3 block(p.threads);
   if (p.kind == kGnRows) {
@@ -852,7 +876,7 @@ extern "C" int lmufft_group_norm(const void* x, int x_dtype, const float* gamma,
 }
 
 extern "C" int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy, int dy_dtype, const float* gamma,
-                                     const float* beta, const int32_t* lengths, const float* stats, int64_t N, int32_t T,
+                                     const float* beta, const int32_t* lengths, const double* stats, int64_t N, int32_t T,
                                      int32_t C, int32_t G, float eps, int act, void* dx, float* dgamma, float* dbeta,
                                      void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "group norm backward";
@@ -868,7 +892,7 @@ extern "C" int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy,
   if (!x || !dy || !gamma || !beta || !dx || (!rows && !stats)) return set_error("%s: NULL pointer", what);
   if (!rows && N > 65535) return set_error("%s: %lld utterances (at most 65535)", what, (long long)N);
   if (!gn_aligned(x) || !gn_aligned(dy) || !gn_aligned(gamma) || !gn_aligned(beta) || !gn_aligned(dx) ||
-      (reinterpret_cast<uintptr_t>(stats) & 7))
+      !gn_aligned(stats))
     return set_error("%s: tensors must start on 16-byte boundaries", what);
   GnPlan p;
   const bool xb = x_dtype == LMUFFT_BF16, gb = dy_dtype == LMUFFT_BF16;
@@ -877,7 +901,7 @@ extern "C" int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy,
   const size_t need = gn_workspace(p, N, C, G, true);
   if (need && (!workspace || workspace_bytes < need || !gn_aligned(workspace)))
     return set_error("%s: workspace of %zu bytes on a 16-byte boundary needed, %zu given", what, need, workspace_bytes);
-  GnArgs a{x,  dy, gamma, beta, lengths, dx, const_cast<float*>(stats), (float*)workspace, eps, (long)N, T, C, G, act,
+  GnArgs a{x,  dy, gamma, beta, lengths, dx, (double2*)const_cast<double*>(stats), (float*)workspace, eps, (long)N, T, C, G, act,
            p.splits, p.split_len};
   const dim3 block(p.threads);
   long partials = N, stride = 2 * C;

@@ -342,13 +342,13 @@ Tensor norm_run(const Tensor& x, const Tensor& weight, const Tensor& bias, const
   const Sample s = sample_of(x);
   Tensor out = at::empty(x.sizes(), x.options().dtype(a.out).requires_grad(false));
   if (with_stats && (s.T > 1 || a.lengths.defined()))
-    *stats = at::empty({s.N, a.groups, 2}, x.options().dtype(at::kFloat).requires_grad(false));
+    *stats = at::empty({s.N, a.groups, 2}, x.options().dtype(at::kDouble).requires_grad(false));
   const size_t bytes = lib.lmufft_group_norm_workspace_bytes(s.N, s.T, s.C, a.groups, 0);
   Tensor ws = workspace(bytes, x);
   OnDevice on(x);
   ran(lib.lmufft_group_norm(x.const_data_ptr(), dtype_of(x), weight.const_data_ptr<float>(), bias.const_data_ptr<float>(),
                             static_cast<const int32_t*>(ptr(a.lengths)), s.N, s.T, s.C, a.groups, (float)a.eps, a.act,
-                            out.mutable_data_ptr(), dtype_of(out), with_stats ? ptr_mut<float>(*stats) : nullptr, ptr_mut<void>(ws), bytes,
+                            out.mutable_data_ptr(), dtype_of(out), with_stats ? ptr_mut<double>(*stats) : nullptr, ptr_mut<void>(ws), bytes,
                             on.stream),
       "lmufft_group_norm");
   return out;
@@ -393,7 +393,7 @@ struct GroupNormTrain : torch::autograd::Function<GroupNormTrain> {
       OnDevice on(x);
       ran(lib.lmufft_group_norm_bwd(x.const_data_ptr(), dtype_of(x), dy.const_data_ptr(), dtype_of(dy), w.const_data_ptr<float>(),
                                     b.const_data_ptr<float>(), static_cast<const int32_t*>(ptr(lengths)),
-                                    static_cast<const float*>(ptr(stats)), s.N, s.T, s.C, groups, (float)ctx->saved_data["eps"].toDouble(),
+                                    static_cast<const double*>(ptr(stats)), s.N, s.T, s.C, groups, (float)ctx->saved_data["eps"].toDouble(),
                                     (int)ctx->saved_data["act"].toInt(), out[0].mutable_data_ptr(), out[1].mutable_data_ptr<float>(),
                                     out[2].mutable_data_ptr<float>(), ptr_mut<void>(ws), bytes, on.stream),
           "lmufft_group_norm_bwd");

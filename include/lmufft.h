@@ -494,16 +494,16 @@ int lmufft_decay_attention_step(const void* q, const void* k, const void* v, int
  * inside the length and the C / G channels of a group.  act: 0 none, 1 ReLU, 2 SiLU.  lengths [N] (NULL: all T frames)
  * is clamped to [0, T]; frames behind it are not read, their outputs and gradients are zeros.
  * C at most 1024, gamma, beta f32 [C], tensors start on 16-byte boundaries; statistics and sums in f32, fixed order.
- *   lmufft_group_norm: out f32 or bf16; stats [N][G][2] f32 (mean, rstd; may be NULL; not written for T = 1 without lengths) is
+ *   lmufft_group_norm: out f32 or bf16; stats [N][G][2] f64 (mean, rstd; may be NULL; not written for T = 1 without lengths) is
  *   what the backward reads.  In place (out == x) is fine with one dtype.
  *   lmufft_group_norm_bwd: dx (dtype of x), dgamma, dbeta f32 [C] (zeros for an empty x).
  * ---------------------------------------------------------------------- */
 size_t lmufft_group_norm_workspace_bytes(int64_t N, int32_t T, int32_t C, int32_t G, int backward);
 int lmufft_group_norm(const void* x, int x_dtype, const float* gamma, const float* beta, const int32_t* lengths,
                       int64_t N, int32_t T, int32_t C, int32_t G, float eps, int act, void* out, int out_dtype,
-                      float* stats, void* workspace, size_t workspace_bytes, void* stream);
+                      double* stats, void* workspace, size_t workspace_bytes, void* stream);
 int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy, int dy_dtype, const float* gamma,
-                          const float* beta, const int32_t* lengths, const float* stats, int64_t N, int32_t T,
+                          const float* beta, const int32_t* lengths, const double* stats, int64_t N, int32_t T,
                           int32_t C, int32_t G, float eps, int act, void* dx, float* dgamma, float* dbeta,
                           void* workspace, size_t workspace_bytes, void* stream);
 

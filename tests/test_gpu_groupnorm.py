@@ -143,6 +143,34 @@ def test_large_offsets_keep_their_variance():
         assert float((got - ref).abs().max()) <= 1000 * U * sums * 2
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,groups", [((200, 384), 6), ((300, 60), 4), ((3, 400, 384), 32), ((2, 3000, 96), 2)])
+def test_the_border_of_the_relu_is_decided_exactly(shape, groups, dtype):
+    """Biases that put one element of each channel within a rounding of zero (2^-25 of the bias, far inside what 32 bits can
+    tell): its slope is the sign's all the same.  The statistics are exact to 64 bits; every such z is above 1e-13."""
+    from asr_amd.groupnorm import group_norm_train
+
+    dev = _dev()
+    C = shape[-1]
+    x, w, _, _ = _make(shape, dtype, 77)
+    hat, *_ = _pieces(x.double(), groups, w.double(), torch.zeros(C, dtype=torch.float64), None)
+    g = torch.Generator().manual_seed(5)
+    rows = hat.reshape(-1, C)
+    at = torch.randint(0, rows.shape[0], (C,), generator=g)
+    cols = torch.arange(C)
+    b = (-rows[at, cols] * w.double()).float()
+    z = rows[at, cols] * w.double() + b.double()
+    assert (z.abs() > 1e-13).all() and (z.abs() < 1e-6).all() and 0.2 < float((z > 0).double().mean()) < 0.8
+    dy = torch.zeros(rows.shape)
+    dy[at, cols] = 1.0
+    leaves = [x.to(dev).requires_grad_(True), w.to(dev).requires_grad_(True), b.to(dev).requires_grad_(True)]
+    y = group_norm_train(leaves[0], groups, *leaves[1:], 1e-5, "relu")
+    dx, dw, db = torch.autograd.grad(y, leaves, dy.reshape(shape).to(dtype).to(dev))
+    assert torch.equal(db.cpu(), (z > 0).float())
+    rx, rw, _ = go.group_norm_backward(x, groups, w, b, dy.reshape(shape), 1e-5, "relu")
+    assert ((dw.double().cpu() - rw).abs() <= 200 * U * rw.abs() + 200 * U * 8).all()  # (one term a channel; |xhat| below 8)
+
+
 @pytest.mark.parametrize("poison", [float("nan"), float("inf")])
 def test_padding_is_not_read(poison):
     from asr_amd.groupnorm import group_norm_train

@@ -14,8 +14,8 @@
 //     threads by shuffles when they are a power of two, through LDS otherwise.
 //   utterances, columns: where an utterance's frames of a few groups fit a workgroup's registers, it reads them once, keeps
 //     them, and writes the result: one launch, one read, one write.
-//   utterances, splits: otherwise the frames are split over workgroups.  k_gn_stats leaves (count, mean, centred second
-//     moment) of each split and group, k_gn_apply joins them and normalises, reading x again.  The backward does the same
+//   utterances, splits: otherwise the frames are split over workgroups.  k_gn_stats leaves the sums of each split and group,
+//     k_gn_apply joins them and normalises, reading x again.  The backward does the same
 //     with the per-channel sums of dz and dz xhat, from which the group sums and the parameter gradients both follow.
 // Second moments are taken about a value of the data, never as a difference of large sums.  The utterances' statistics are
 // summed in 64 bits, everything else in 32.  Fixed order, no atomics.  HBM-bound.
@@ -31,7 +31,7 @@
 namespace lmufft {
 
 constexpr int kGnMaxWidth = 1024;
-constexpr int kGnMaxSplits = 64;
+constexpr int kGnMaxSplits = 256;
 constexpr int kGnRowBwdBlocks = 1024;  // workgroups of the rows backward: each leaves one partial of the parameter gradients
 
 enum { kGnNone = 0, kGnRelu = 1, kGnSilu = 2 };
@@ -327,28 +327,12 @@ __global__ __launch_bounds__(1024) void k_gn_rows_bwd(GnArgs a) {
   gn_channel_sums<V>(dg, db, TR, RB, on ? slot : -1, gn_sums, [&](int which, int i, float s) { out[which * a.C + i] = s; });
 }
 
-// (count, mean, M2) of a set of values, and of two disjoint sets together.  Joined in 64 bits: a handful of values a
-// group, and what they lose would shift every value of the group.
-struct GnMoment {
-  double n, mean, m2;
-};
-__device__ __forceinline__ GnMoment gn_join(const GnMoment& p, const GnMoment& q) {
-  const double n = p.n + q.n;
-  if (n == 0.) return p;
-  const double d = q.mean - p.mean, w = q.n / n;
-  return GnMoment{n, p.mean + d * w, p.m2 + q.m2 + d * d * p.n * w};
-}
-
 __device__ __forceinline__ int gn_len(const GnArgs& a, long n) { return a.lengths ? min(max(a.lengths[n], 0), a.T) : a.T; }
 
-// The moments of cnt values from the sum and the sum of squares of their distances from a pivot.
-__device__ __forceinline__ GnMoment gn_moment(double cnt, float pivot, double s, double ss) {
-  if (cnt <= 0.) return GnMoment{0., 0., 0.};
-  const double m2 = ss - s * s / cnt;
-  return GnMoment{cnt, pivot + s / cnt, m2 < 0. ? 0. : m2};
-}
-__device__ __forceinline__ double2 gn_mean_rstd(const GnMoment& t, float eps) {
-  return make_double2(t.mean, 1. / sqrt((t.n > 0. ? t.m2 / t.n : 0.) + (double)eps));
+// Mean and 1 / standard deviation of cnt values from the sum and the sum of squares of their distances from a pivot.
+__device__ __forceinline__ double2 gn_mean_rstd(double cnt, float pivot, double s, double ss, float eps) {
+  const double m = cnt > 0. ? s / cnt : 0., var = cnt > 0. ? ss / cnt - m * m : 0.;
+  return make_double2(pivot + m, 1. / sqrt((var < 0. ? 0. : var) + (double)eps));
 }
 // A vector's part of the sums about the pivot, in 64 bits: memory is waited for anyway, and the ReLU's border asks for a mean
 // that is exact (gn_slope).
@@ -384,8 +368,8 @@ __device__ __forceinline__ GnVec<V> gn_dx(const GnVec<V>& x, const GnVec<V>& dy,
 
 // ---- utterances.  Threads of a row own V channels each, the workgroup's rows of threads take its frames in turn.
 //
-// Sums of a group: (sum, sum of squares) of x - pivot over the threads of the group, the pivot being one value of the group
-// that all its threads take, so the partials of a workgroup simply add up.  red: one double2 a thread.  The threads
+// Sums of a group: (sum, sum of squares) of x - pivot over the threads of the group, the pivot being the group's first value in
+// the utterance, which all take, so partials simply add up.  red: one double2 a thread.  The threads
 // tid / lanes, each team of `lanes` (a power of two up to 64) joining one group at a time, call `put(group, sum, squares)`.
 template <class F>
 __device__ __forceinline__ void gn_join_groups(double s, double ss, int TR, int RB, int L, int G, double2* red, F put) {
@@ -412,7 +396,7 @@ __device__ __forceinline__ void gn_join_groups(double s, double ss, int TR, int 
   }
 }
 
-// Workgroup (split, n) of the statistics over several workgroups: each split's moments of each group.
+// Workgroup (split, n) of the statistics over several workgroups: each split's sums of each group, part[n][split][G].
 template <bool XB, int V>
 __global__ __launch_bounds__(1024) void k_gn_stats(GnArgs a) {
   __shared__ double2 red[1024];
@@ -423,19 +407,15 @@ __global__ __launch_bounds__(1024) void k_gn_stats(GnArgs a) {
   const long base = n * a.T * a.C;
   double s = 0., ss = 0.;
   if (slot < RB && t0 < t1) {
-    const float pivot = gn_load<XB, 1>(a.x, base + (long)t0 * a.C + c / cg * cg).f[0];
+    const float pivot = gn_load<XB, 1>(a.x, base + c / cg * cg).f[0];
 #pragma unroll 4
     for (int t = t0 + slot; t < t1; t += RB) {
       const GnVec<V> x = gn_load<XB, V>(a.x, base + (long)t * a.C + c);
       gn_add_moments<V>(x, pivot, s, ss);
     }
   }
-  GnMoment* const out = reinterpret_cast<GnMoment*>(a.part) + (n * a.splits + blockIdx.x) * a.G;
-  gn_join_groups(s, ss, TR, RB, L, a.G, red, [&](int g, double u, double v) {
-    const double cnt = (double)max(t1 - t0, 0) * cg;
-    const float pivot = cnt > 0. ? gn_load<XB, 1>(a.x, base + (long)t0 * a.C + g * cg).f[0] : 0.f;
-    out[g] = gn_moment(cnt, pivot, u, v);
-  });
+  double2* const out = reinterpret_cast<double2*>(a.part) + (n * a.splits + blockIdx.x) * a.G;
+  gn_join_groups(s, ss, TR, RB, L, a.G, red, [&](int g, double u, double v) { out[g] = make_double2(u, v); });
 }
 
 template <bool XB, bool OB, int V>
@@ -444,17 +424,33 @@ __global__ __launch_bounds__(1024) void k_gn_apply(GnArgs a) {
   const int TR = a.C / V, RB = blockDim.x / TR, cg = a.C / a.G;
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V;
   const long n = blockIdx.y;
-  for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
-    GnMoment t{0., 0., 0.};
-    for (int s = 0; s < a.splits; ++s) t = gn_join(t, *(reinterpret_cast<const GnMoment*>(a.part) + (n * a.splits + s) * a.G + g));
-    st[g] = gn_mean_rstd(t, a.eps);
-    if (a.stats && blockIdx.x == 0) a.stats[n * a.G + g] = st[g];
+  const int len = gn_len(a, n);
+  // a group's splits are summed by a team of lanes (one thread a group took 0.8 us a split)
+  int lanes = 1;
+  while (lanes < 64 && lanes < a.splits) lanes <<= 1;
+  for (int g0 = 0; g0 < a.G; g0 += blockDim.x / lanes) {  // uniform: the shuffles need every lane
+    const int g = g0 + threadIdx.x / lanes, lane = threadIdx.x % lanes;
+    double s = 0., ss = 0.;
+    if (g < a.G)
+      for (int i = lane; i < a.splits; i += lanes) {
+        const double2 p = reinterpret_cast<const double2*>(a.part)[(n * a.splits + i) * a.G + g];
+        s += p.x;
+        ss += p.y;
+      }
+    for (int o = lanes >> 1; o > 0; o >>= 1) {
+      s += __shfl_xor(s, o);
+      ss += __shfl_xor(ss, o);
+    }
+    if (g < a.G && lane == 0) {
+      st[g] = gn_mean_rstd((double)len * cg, len > 0 ? gn_load<XB, 1>(a.x, n * a.T * a.C + g * cg).f[0] : 0.f, s, ss, a.eps);
+      if (a.stats && blockIdx.x == 0) a.stats[n * a.G + g] = st[g];
+    }
   }
   __syncthreads();
   if (slot >= RB) return;
   const GnVec<V> g = gn_load<false, V>(a.gamma, c), bt = gn_load<false, V>(a.beta, c);
   const GnStat st_ = gn_stat(st[c / cg]);
-  const int len = gn_len(a, n), t0 = blockIdx.x * a.split_len, t1 = min(t0 + a.split_len, a.T);
+  const int t0 = blockIdx.x * a.split_len, t1 = min(t0 + a.split_len, a.T);
   const long base = n * a.T * a.C + c;
 #pragma unroll 4
   for (int t = t0 + slot; t < min(t1, len); t += RB) {
@@ -498,28 +494,31 @@ __global__ __launch_bounds__(1024) void k_gn_bwd_sums(GnArgs a) {
   gn_channel_sums<V>(dg, db, TR, RB, on ? slot : -1, gn_sums, [&](int which, int i, float s) { out[which * a.C + i] = s; });
 }
 
-// A sample's splits joined: its channel sums in the place of its first split's, and its groups' means
-// (sum gamma dz) / n, (sum gamma dz xhat) / n behind all partials.
+// A sample's splits joined, by workgroups of a few groups each: its channel sums in the place of its first split's, and its
+// groups' means (sum gamma dz) / n, (sum gamma dz xhat) / n behind all partials.
 __global__ __launch_bounds__(1024) void k_gn_bwd_join(GnArgs a) {
   __shared__ float sums[2 * kGnMaxWidth];
   const long n = blockIdx.x;
   const int cg = a.C / a.G, len = gn_len(a, n);
+  const int g0 = (int)((long)a.G * blockIdx.y / gridDim.y), g1 = (int)((long)a.G * (blockIdx.y + 1) / gridDim.y);
+  const int c0 = g0 * cg, width = (g1 - g0) * cg;
   float* const p = a.part + n * a.splits * 2 * a.C;
-  for (int i = threadIdx.x; i < 2 * a.C; i += blockDim.x) {
+  for (int i = threadIdx.x; i < 2 * width; i += blockDim.x) {
+    const int c = c0 + (i < width ? i : i - width), at = i < width ? c : a.C + c;
     float t = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) t += p[(long)s * 2 * a.C + i];
-    p[i] = t;
-    sums[i] = t * a.gamma[i < a.C ? i : i - a.C];
+#pragma unroll 16
+    for (int s = 0; s < a.splits; ++s) t += p[(long)s * 2 * a.C + at];
+    p[at] = t;
+    sums[i] = t * a.gamma[c];
   }
   __syncthreads();
   float2* const out = reinterpret_cast<float2*>(a.part + a.N * a.splits * 2 * a.C) + n * a.G;
   const float inv = len > 0 ? 1.f / ((float)len * (float)cg) : 0.f;
-  for (int g = threadIdx.x >> 6; g < a.G; g += blockDim.x >> 6) {
+  for (int g = threadIdx.x >> 6; g < g1 - g0; g += blockDim.x >> 6) {
     float s1 = 0.f, s2 = 0.f;
-    for (int i = g * cg + (threadIdx.x & 63); i < (g + 1) * cg; i += 64) s1 += sums[a.C + i], s2 += sums[i];
+    for (int i = g * cg + (threadIdx.x & 63); i < (g + 1) * cg; i += 64) s1 += sums[width + i], s2 += sums[i];
     for (int o = 32; o > 0; o >>= 1) s1 += __shfl_xor(s1, o), s2 += __shfl_xor(s2, o);
-    if ((threadIdx.x & 63) == 0) out[g] = make_float2(s1 * inv, s2 * inv);
+    if ((threadIdx.x & 63) == 0) out[g0 + g] = make_float2(s1 * inv, s2 * inv);
   }
 }
 
@@ -586,7 +585,7 @@ __global__ __launch_bounds__(1024) void k_gn_column(GnArgs a) {
   gn_join_groups(s, ss, TR, RB, L, groups, red, [&](int g, double u, double v) {
     const int frames = gn_len(a, n);
     const float p = frames > 0 ? gn_load<XB, 1>(a.x, first + g * cg).f[0] : 0.f;
-    st[g] = gn_mean_rstd(gn_moment((double)frames * cg, p, u, v), a.eps);
+    st[g] = gn_mean_rstd((double)frames * cg, p, u, v, a.eps);
     if (a.stats) a.stats[n * a.G + block * groups + g] = st[g];
   });
   __syncthreads();
@@ -769,8 +768,9 @@ static bool gn_plan(int64_t N, int32_t T, int32_t C, int32_t G, bool wide, bool 
     return true;
   }
   p->kind = kGnSplit;
-  // about 2048 workgroups in all, each with at least eight frames for a thread
-  long s = std::max<long>(1, 2048 / std::max<long>(1, N));
+  // about 4096 workgroups in all, each with at least eight frames for a thread (32 x 2999 x 384 f32, lengths from a tenth up:
+  // 2048 184 us of kernels forward and backward, 4096 177, 8192 178)
+  long s = std::max<long>(1, 4096 / std::max<long>(1, N));
   s = std::min<long>(std::min<long>(s, kGnMaxSplits), std::max<long>(1, T / (8L * rb)));
   p->split_len = (int)((T + s - 1) / s);
   p->splits = p->split_len ? (T + p->split_len - 1) / p->split_len : 1;
@@ -779,7 +779,7 @@ static bool gn_plan(int64_t N, int32_t T, int32_t C, int32_t G, bool wide, bool 
 static size_t gn_workspace(const GnPlan& p, int64_t N, int32_t C, int32_t G, bool backward) {
   if (p.kind == kGnRows) return backward ? sizeof(float) * 2 * C * (size_t)p.blocks : 0;
   if (p.kind == kGnColumn) return backward ? sizeof(float) * 2 * C * (size_t)N : 0;
-  return backward ? sizeof(float) * 2 * ((size_t)N * p.splits * C + (size_t)N * G) : sizeof(GnMoment) * (size_t)N * p.splits * G;
+  return backward ? sizeof(float) * 2 * ((size_t)N * p.splits * C + (size_t)N * G) : sizeof(double2) * (size_t)N * p.splits * G;
 }
 static dim3 gn_column_grid(const GnPlan& p, int64_t N) { return dim3((unsigned)((N + 7) / 8 * 8 * p.splits)); }
 
@@ -925,7 +925,7 @@ extern "C" int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy,
     }
     {
       ProfScope ps("k_gn_bwd_join", st);
-      hipLaunchKernelGGL(k_gn_bwd_join, dim3((unsigned)N), dim3(std::min(1024, (2 * C + 63) / 64 * 64)), 0, st, a);
+      hipLaunchKernelGGL(k_gn_bwd_join, dim3((unsigned)N, std::min(G, 8)), dim3(256), 0, st, a);
     }
     ProfScope ps("k_gn_bwd_apply", st);
     GN_BY_2(xb, gb, GN_BY_V(p.V, hipLaunchKernelGGL((k_gn_bwd_apply<A, B, V>), grid, block, 0, st, a)));

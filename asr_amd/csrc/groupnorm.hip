@@ -32,6 +32,7 @@ namespace lmufft {
 
 constexpr int kGnMaxWidth = 1024;
 constexpr int kGnMaxSplits = 256;
+constexpr int kGnFrames = 16, kGnBwdFrames = 10;  // frames a thread of the column kernels can keep (or eight)
 constexpr int kGnRowBwdBlocks = 1024;  // workgroups of the rows backward: each leaves one partial of the parameter gradients
 
 enum { kGnNone = 0, kGnRelu = 1, kGnSilu = 2 };
@@ -714,9 +715,10 @@ struct GnPlan {
 };
 
 // The smallest workgroup whose threads keep the T frames of `width` channels, eight frames each where that is enough, at most
-// 16 or what 64 registers hold (`words`: half registers of a kept value: x as it lies in memory, and dz).  False if none does.
-static bool gn_column_fits(int T, int width, int V, int words, GnPlan* p) {
-  const int tc = width / V, most = std::min(16, 128 / (V * words));
+// what the kernels have room for, or what 64 registers hold (`words`: half registers of a kept value: x as it lies in memory,
+// and dz).  False if none does.
+static bool gn_column_fits(int T, int width, int V, int words, bool backward, GnPlan* p) {
+  const int tc = width / V, most = std::min(backward ? kGnBwdFrames : kGnFrames, 128 / (V * words));
   for (int least : {8, 16})
     for (int threads : {256, 512, 1024}) {
       if (tc > threads) continue;
@@ -754,14 +756,15 @@ static bool gn_plan(int64_t N, int32_t T, int32_t C, int32_t G, bool wide, bool 
   for (int m = 1; m <= G; ++m) {
     if (G % m) continue;
     const int w = m * cg;
-    if (!gn_column_fits(T, w, q.V, words, &q)) break;
+    if (!gn_column_fits(T, w, q.V, words, backward, &q)) break;
     if (m > least && N * (G / m) < 512) break;
     best = m;
     if (m >= least && w * x_bytes >= 128) break;
   }
-  if (best && (N * (G / best) >= 192 || (size_t)T * best * cg <= 16 * 1024)) {
+  // (HIP counts a launch's threads in 32 bits)
+  if (best && (N + 8) * (G / best) < (1L << 22) && (N * (G / best) >= 192 || (size_t)T * best * cg <= 16 * 1024)) {
     p->V = q.V;
-    gn_column_fits(T, best * cg, p->V, words, p);
+    gn_column_fits(T, best * cg, p->V, words, backward, p);
     p->kind = kGnColumn;
     p->splits = G / best;
     p->split_len = best * cg;
@@ -860,7 +863,7 @@ extern "C" int lmufft_group_norm(const void* x, int x_dtype, const float* gamma,
   } else if (p.kind == kGnColumn) {
     ProfScope ps("k_gn_column", st);
     if (p.frames <= 8) GN_BY_2(xb, ob, GN_BY_V4(p.V, hipLaunchKernelGGL((k_gn_column<A, B, V, 8>), gn_column_grid(p, N), block, 0, st, a)));
-    else GN_BY_2(xb, ob, GN_BY_V4(p.V, hipLaunchKernelGGL((k_gn_column<A, B, V, 16>), gn_column_grid(p, N), block, 0, st, a)));
+    else GN_BY_2(xb, ob, GN_BY_V4(p.V, hipLaunchKernelGGL((k_gn_column<A, B, V, kGnFrames>), gn_column_grid(p, N), block, 0, st, a)));
   } else {
     const dim3 grid(p.splits, (unsigned)N);
     {
@@ -915,7 +918,7 @@ extern "C" int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy,
   } else if (p.kind == kGnColumn) {
     ProfScope ps("k_gn_column_bwd", st);
     if (p.frames <= 8) GN_BY_2(xb, gb, GN_BY_V4(p.V, hipLaunchKernelGGL((k_gn_column_bwd<A, B, V, 8>), gn_column_grid(p, N), block, lds, st, a)));
-    else GN_BY_2(xb, gb, GN_BY_V4(p.V, hipLaunchKernelGGL((k_gn_column_bwd<A, B, V, 10>), gn_column_grid(p, N), block, lds, st, a)));
+    else GN_BY_2(xb, gb, GN_BY_V4(p.V, hipLaunchKernelGGL((k_gn_column_bwd<A, B, V, kGnBwdFrames>), gn_column_grid(p, N), block, lds, st, a)));
   } else {
     stride *= p.splits;
     const dim3 grid(p.splits, (unsigned)N);

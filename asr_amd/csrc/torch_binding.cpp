@@ -75,7 +75,9 @@ Tensor frames_of(const char* what, const char* name, const MaybeTensor& counts, 
   if (!counts.has_value() || !counts->defined()) return Tensor();
   TORCH_CHECK(counts->dim() == 1 && counts->size(0) == batch, what, ": `", name, "` must have shape (", batch, ",), got ", counts->sizes());
   TORCH_CHECK(!counts->is_floating_point() && !counts->is_complex(), what, ": `", name, "` must hold whole numbers, got ", counts->scalar_type());
-  return counts->to(like.device(), at::kInt).contiguous();
+  // what does not fit 32 bits keeps its meaning
+  const Tensor fit = counts->scalar_type() == at::kLong ? counts->clamp(0, INT32_MAX) : *counts;
+  return fit.to(like.device(), at::kInt).contiguous();
 }
 
 Tensor workspace(size_t bytes, const Tensor& like) {

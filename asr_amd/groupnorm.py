@@ -25,7 +25,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor, bias: tor
 
     x: float32 or bfloat16; weight, bias: [C].  activation: None, "relu" or "silu".  lengths [B]: frames of each utterance
     (whole numbers, clamped to [0, T]).  The result has `out_dtype`, by default float32 under autocast (where torch runs its
-    norms in float32) and the input's dtype otherwise.  At most 1024 channels."""
+    norms in float32) and the input's dtype otherwise.  At most 1024 channels, and 65535 utterances (rows: any number)."""
     return ops.group_norm(x, num_groups, weight, bias, eps, activation, lengths, out_dtype)
 
 

@@ -81,6 +81,14 @@ CASES = [
     ((2, 257, 1000), 8, [257, 256]),
     ((4, 130, 250), 2, [130, 129, 2, 1]),
     ((70, 50, 64), 1, None),
+    # odd groups of long utterances: as many frames a thread as the kernels keep, and more than that
+    ((2, 1000, 30), 2, [1000, 999]),
+    ((1, 700, 18), 2, None),
+    ((3, 680, 30), 2, [680, 1, 341]),
+    ((2, 1100, 30), 2, None),
+    ((110, 500, 10), 5, None),
+    ((2, 2600, 12), 2, [2600, 2599]),
+    ((200, 170, 36), 3, None),
 ]
 
 
@@ -256,6 +264,15 @@ def test_captured_training_pass_replays():
         torch.cuda.synchronize()
         for a, r in zip(got, go_()):
             assert torch.equal(a, r), i
+
+
+def test_lengths_of_64_bits():
+    from asr_amd.groupnorm import group_norm
+
+    dev = _dev()
+    x, w, b, _ = (t.to(dev) for t in _make((3, 20, 96), torch.float32, 4))
+    ref = group_norm(x, 4, w, b, lengths=torch.tensor([20, 0, 7], dtype=torch.int32, device=dev))
+    assert torch.equal(group_norm(x, 4, w, b, lengths=torch.tensor([1 << 40, -(1 << 40), 7])), ref)
 
 
 def test_empty_calls_and_refusals():

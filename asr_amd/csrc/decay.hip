@@ -110,7 +110,8 @@ static int decay_check(const char* what, int dtype, int32_t B, int32_t T, int32_
   if (dtype != LMUFFT_F32 && dtype != LMUFFT_BF16) return set_error("%s: unknown dtype %d", what, dtype);
   if (B < 0 || T < 0 || H <= 0) return set_error("%s: bad shape (B=%d T=%d H=%d)", what, B, T, H);
   if (!decay_width(dk) || !decay_width(dv)) return set_error("%s: head widths %d, %d (supported: 32, 64, 128)", what, dk, dv);
-  if ((long)B * H > 0x7fffffffL || T > (1 << 26)) return set_error("%s: too large (B=%d T=%d H=%d)", what, B, T, H);
+  // (HIP counts a launch's threads in 32 bits, 512 for each head; and the kernels an utterance's 16-byte pieces)
+  if ((long)B * H >= (1 << 23) || T > (1 << 25)) return set_error("%s: too large (B=%d T=%d H=%d)", what, B, T, H);
   return 0;
 }
 

@@ -222,6 +222,8 @@ __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k
   constexpr int PIECES_K = C * DK / VEC, PIECES_V = C * DV / VEC;  // 16-byte pieces of the tiles, and how many a thread stages
   constexpr int NK = (PIECES_K + THREADS - 1) / THREADS, NV = (PIECES_V + THREADS - 1) / THREADS;
   extern __shared__ __attribute__((aligned(16))) unsigned char dec_lds[];
+  // OUT: from which frame on a column is NaN, because v holds an infinity or a NaN there
+  __shared__ int odd_from[DV], odd_any;
   const DecTile<T, DK> ktile{reinterpret_cast<T*>(dec_lds)};  // [C][DK]
   const DecTile<T, DV> vtile{ktile.base + C * DK};            // [C][DV]
   const DecTile<T, DK> qtile{vtile.base + C * DV};            // [C][DK]
@@ -322,8 +324,11 @@ __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k
       *reinterpret_cast<dec_u4*>(vtile.piece(vrow(n), vpiece(n))) = f.v[n];
     }
   };
+  if (OUT) {
+    if (tid == 0) odd_any = 0;
+    for (int i = tid; i < DV; i += THREADS) odd_from[i] = 0x7fffffff;
+  }
   Rows rows;  // one chunk ahead (two ahead measured the same, in twice the registers)
-  if (s0 < end) fetch(s0, rows);
 
   const float a2 = dec_log2(args.log_decay[h]);
   auto upow = [&](int n) { return dec_uniform(dec_pow(a2, n)); };
@@ -337,6 +342,7 @@ __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k
     if (t0 + C < end) fetch(t0 + C, rows);
   };
 
+  if (s0 < end) fetch(s0, rows);
   if (!holds) {
     float wdiag[4], woff[4];  // lambda^(i-j) inside a tile, and 16 more: tile by tile times a uniform power
 #pragma unroll
@@ -353,37 +359,59 @@ __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k
       Frag qx[KB];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) qx[kb] = qtile.row_frag(16 * it + l16, kb, g);
+      // The products carry an infinity or a NaN in v to the frames before it, too (zero times infinity).  A wave that finds such
+      // an output puts zeros in their place in the tile, notes from where on their columns are NaN (these are written at the
+      // end) and computes the chunk once more.  What another wave reads meanwhile does not matter: its outputs are finite, or it
+      // does the same, and the state's column is one of those noted.
       dec_f4 o[MO];
+      for (bool again = false;; again = true) {
 #pragma unroll
-      for (int i = 0; i < MO; ++i) {
-        o[i] = dec_f4(0.f);
+        for (int i = 0; i < MO; ++i) {
+          o[i] = dec_f4(0.f);
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) o[i] = dec_mma(stile.row_frag(16 * (mo0 + i) + l16, kb, g), qx[kb], o[i]);
-        o[i] *= fq;
-      }
-#pragma unroll 1
-      for (int jb = 0; jb <= it >> 1; ++jb) {
-        dec_f4 p[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int jt = 2 * jb + x;
-          p[x] = dec_f4(0.f);
-          if (jt > it) continue;
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb) p[x] = dec_mma(ktile.row_frag(16 * jt + l16, kb, g), qx[kb], p[x]);
-          if (jt == it) {  // masked by selection: a frame behind this one contributes nothing, whatever it holds
-#pragma unroll
-            for (int r = 0; r < 4; ++r) p[x][r] = l16 >= 4 * g + r ? p[x][r] * wdiag[r] : 0.f;
-          } else {
-            const float far = upow(16 * (it - jt - 1));
-#pragma unroll
-            for (int r = 0; r < 4; ++r) p[x][r] *= woff[r] * far;
-          }
+          for (int kb = 0; kb < KB; ++kb) o[i] = dec_mma(stile.row_frag(16 * (mo0 + i) + l16, kb, g), qx[kb], o[i]);
+          o[i] *= fq;
         }
-        Frag pf;
-        dec_pack(pf, p[0], p[1]);
+#pragma unroll 1
+        for (int jb = 0; jb <= it >> 1; ++jb) {
+          dec_f4 p[2];
 #pragma unroll
-        for (int i = 0; i < MO; ++i) o[i] = dec_mma(vtile.col_frag(32 * jb, 16 * (mo0 + i), l16, g), pf, o[i]);
+          for (int x = 0; x < 2; ++x) {
+            const int jt = 2 * jb + x;
+            p[x] = dec_f4(0.f);
+            if (jt > it) continue;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) p[x] = dec_mma(ktile.row_frag(16 * jt + l16, kb, g), qx[kb], p[x]);
+            if (jt == it) {  // masked by selection: a frame behind this one contributes nothing, whatever it holds
+#pragma unroll
+              for (int r = 0; r < 4; ++r) p[x][r] = l16 >= 4 * g + r ? p[x][r] * wdiag[r] : 0.f;
+            } else {
+              const float far = upow(16 * (it - jt - 1));
+#pragma unroll
+              for (int r = 0; r < 4; ++r) p[x][r] *= woff[r] * far;
+            }
+          }
+          Frag pf;
+          dec_pack(pf, p[0], p[1]);
+#pragma unroll
+          for (int i = 0; i < MO; ++i) o[i] = dec_mma(vtile.col_frag(32 * jb, 16 * (mo0 + i), l16, g), pf, o[i]);
+        }
+        dec_f4 odd = dec_f4(0.f);
+#pragma unroll
+        for (int i = 0; i < MO; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) odd[r] = fmaf(o[i][r], 0.f, odd[r]);
+        if (again || __builtin_expect(!__any((odd[0] + odd[1]) + (odd[2] + odd[3]) != 0.f), 1)) break;
+#pragma unroll 1
+        for (int e = lane; e < C * DV; e += 64) {
+          T* const v = vtile.piece(e / DV, e % DV / VEC) + e % VEC;
+          if (__builtin_isfinite((float)*v)) continue;
+          *v = (T)0.f;
+          atomicMin(&odd_from[e % DV], t0 + e / DV);
+          odd_any = 1;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
       }
       const int t = t0 + 16 * it + l16;
       if (t < end) {
@@ -392,6 +420,7 @@ __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k
         for (int i = 0; i < MO; ++i) dec_store4(dst + 16 * i, o[i] * args.scale);
       }
     }
+    __syncthreads();
   } else {
     // ---- the state this segment starts from: tile (t, m), this lane: column scol + 16 m + l16, rows srow + 16 t + 4 g + r
     dec_f4 S[KT][MS];
@@ -478,6 +507,7 @@ __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k
       }
     }
 
+    if (OUT) __syncthreads();
     if (!OUT) {
       dec_f4* e = reinterpret_cast<dec_f4*>(R.ws + ((long)bh * args.segments + seg) * (DK * DV)) + wplace;
 #pragma unroll
@@ -492,10 +522,18 @@ __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k
 #pragma unroll
         for (int m = 0; m < MS; ++m)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sp[(16 * t + r) * DV + 16 * m] = S[t][m][r];
+          for (int r = 0; r < 4; ++r)
+            sp[(16 * t + r) * DV + 16 * m] = odd_from[scol + 16 * m + l16] < end ? __builtin_nanf("") : S[t][m][r];
     }
   }
   if (!OUT) return;
+  if (odd_any) {
+    for (int i = tid; i < (end - s0) * DV; i += THREADS) {
+      const int t = s0 + i / DV, c = i % DV;
+      if (t >= odd_from[c])
+        ((T*)R.out.p)[(long)b * R.out.bs + (long)(rev ? len - 1 - t : t) * R.out.ld + (long)h * DV + c] = (T)__builtin_nanf("");
+    }
+  }
   // zeros behind the utterance's end
   for (int i = max(s0, len) * (DV / VEC) + tid; i < s1 * (DV / VEC); i += THREADS) {
     const int t = i / (DV / VEC), c = (i % (DV / VEC)) * VEC;

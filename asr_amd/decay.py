@@ -14,9 +14,9 @@ masked_attention takes (asr_amd/attention.py), but is causal: frame t sees the f
     decay_attention_train_packed  the same on q | k | v as the column blocks of one projection's output
 
 Frames from an utterance's length on are padding: whatever they hold, they are not read, their outputs and gradients are
-zeros, and the state is the one behind the last frame inside.  (A frame INSIDE the length that holds inf or NaN spreads it
-to all later frames, and may spread it to the up to 63 frames before it that share its chunk.)  The decays are constants of
-the model: no gradient is returned for them, and the backward has no backward of its own.
+zeros, and the state is the one behind the last frame inside.  An infinity or a NaN inside the length reaches the frames from
+its own on (an infinity may come out as a NaN there), and none before.  The decays are constants of the model: no gradient is
+returned for them, and the backward has no backward of its own.
 """
 from __future__ import annotations
 

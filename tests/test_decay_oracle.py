@@ -93,7 +93,8 @@ def test_c_entry_points_refuse_before_any_launch():
                        (dict(B=-1), b"bad shape"), (dict(H=0), b"bad shape"), (dict(q=None), b"`q` is NULL"),
                        (dict(ld=130), b"16-byte"), (dict(q=ctypes.c_void_p(4104)), b"16-byte"), (dict(ld=-128), b"negative"),
                        (dict(ldo=64), b"overlap"), (dict(dec=None), b"log_decay"), (dict(st=ctypes.c_void_p(4100)), b"`state`"),
-                       (dict(T=4000, B=1), b"workspace"), (dict(T=1 << 27), b"too large")):
+                       (dict(T=4000, B=1), b"workspace"), (dict(T=1 << 27), b"too large"), (dict(T=(1 << 25) + 1, B=1), b"too large"),
+                       (dict(B=1 << 22, H=2, T=1), b"too large")):
         assert fwd(**call) != 0 and text in lib.lmufft_last_error(), (call, lib.lmufft_last_error())
     assert fwd(B=0) == 0 and fwd(T=0) == 0
     assert lib.lmufft_decay_workspace_bytes(_lib.BF16, 1, 4000, 2, 64, 64, 0) > 0

@@ -237,6 +237,54 @@ def test_padding_is_not_read(dtype, poison):
             assert (a[i, n:] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("d,dv,at", [(64, 64, 70), (64, 64, 64), (64, 64, 95), (32, 128, 17), (128, 128, 40), (128, 32, 127)])
+def test_nothing_reaches_an_earlier_frame(d, dv, at, poison, dtype):
+    """An infinity or a NaN inside the length: the frames before it come out bit for bit as without it (and so do the other
+    columns behind it, where it sits in v); gradients run the other way, from an odd dout to no later frame."""
+    from asr_amd.decay import decay_attention, decay_attention_train
+
+    dev = _dev()
+    B, T, H = 2, 200, 2
+    q, k, v, w, _ = (t.to(dev) for t in _make(B, T, H, d, dv, dtype, 19))
+    ld = torch.tensor([-0.01, -0.3], device=dev)
+    clean = decay_attention(q, k, v, H, ld)
+    for which in range(3):
+        bad = [q.clone(), k.clone(), v.clone()]
+        bad[which][1, at, 5] = poison
+        out = decay_attention(*bad, H, ld)
+        assert torch.equal(out[0], clean[0]) and torch.equal(out[1, :at], clean[1, :at])
+        assert torch.equal(out[1, :, dv:], clean[1, :, dv:])  # the other head
+        if which == 0:
+            assert torch.equal(out[1, at + 1:], clean[1, at + 1:]) and not torch.isfinite(out[1, at, :dv]).any()
+        elif which == 1:
+            assert not torch.isfinite(out[1, at:, :dv]).any()
+        else:
+            assert not torch.isfinite(out[1, at:, 5]).any()
+            keep = [c for c in range(dv) if c != 5]
+            assert torch.equal(out[1][:, keep], clean[1][:, keep])
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    ref = torch.autograd.grad(decay_attention_train(*leaves, H, ld), leaves, w)
+    odd = w.clone()
+    odd[1, at, 5] = poison
+    got = torch.autograd.grad(decay_attention_train(*leaves, H, ld), leaves, odd)
+    for a, r, name in zip(got, ref, ("dq", "dk", "dv")):
+        assert torch.equal(a[0], r[0]), name
+        after = slice(at + 1, T) if name != "dq" else [t for t in range(T) if t != at]
+        assert torch.equal(a[1, after], r[1, after]), name
+
+
+def test_lengths_of_64_bits():
+    from asr_amd.decay import decay_attention
+
+    dev = _dev()
+    q, k, v, _, _ = (t.to(dev) for t in _make(3, 40, 2, 32, 32, torch.float32, 6))
+    ld = _decays(2).to(dev)
+    ref = decay_attention(q, k, v, 2, ld, torch.tensor([40, 0, 9], dtype=torch.int32, device=dev))
+    assert torch.equal(decay_attention(q, k, v, 2, ld, torch.tensor([1 << 40, -(1 << 40), 9])), ref)
+
+
 def test_gradients_against_differences():
     """Along a random direction; f32, so a central difference of step h is off by h^2 / 6 of the third derivative -- zero in
     each single operand, in which the operator is linear -- and by rounding, 2^-24 of the sum's magnitudes over h."""
@@ -257,15 +305,15 @@ def test_gradients_against_differences():
         assert abs(float((f(1.0) - f(-1.0)) / 2) - float((grads[i].double() * u.double()).sum())) <= most
 
 
-def test_captured_calls_replay():
+@pytest.mark.parametrize("B,T,H,d", [(2, 700, 2, 64), (1, 300, 3, 128), (1, 1500, 1, 32)])
+def test_captured_calls_replay(B, T, H, d):
     """A prompt and a step captured together, and a training pass: every replay against the eager result, with eager calls
     of the same operators in between."""
     from asr_amd.decay import decay_attention, decay_attention_step, decay_attention_train_packed
 
     dev = _dev()
-    B, T, H, d = 2, 700, 2, 64
     q, k, v, _, st = (t.to(dev) for t in _make(B, T, H, d, d, torch.bfloat16, 31))
-    ld, ln = _decays(H).to(dev), torch.tensor([700, 333], dtype=torch.int32, device=dev)
+    ld, ln = _decays(H).to(dev), torch.tensor([T, T // 2 - 17][:B], dtype=torch.int32, device=dev)
     qkv = torch.cat([q, k, v], -1).requires_grad_(True)
     w = torch.randn_like(q)
 

@@ -230,7 +230,7 @@ extern "C" int lmufft_decay_attention_bwd(const void* q, const void* k, const vo
                   rv = {tk, tq, td, gv, ws ? ws + 2 * part : ws, 1};
   a.role[0] = rq, a.role[1] = rk, a.role[2] = rv;
   if (dk == dv) return decay_launch_any(dtype, a, 3, dk, dv, (hipStream_t)stream);
-  // the other way round the operator's DK is dv; the segments were chosen for chunks that depend on the type alone
+  // the other way round the operator's DK is dv; the chunks the segments were chosen for depend on the sum of the widths
   if (decay_launch_any(dtype, a, 2, dv, dk, (hipStream_t)stream)) return 1;
   a.role[0] = rv;
   return decay_launch_any(dtype, a, 1, dk, dv, (hipStream_t)stream);

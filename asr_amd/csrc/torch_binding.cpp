@@ -101,7 +101,7 @@ struct Rows {  // a [B][T][width] tensor with rows the kernels can load 16 bytes
 };
 bool rows_fit(const Tensor& t) {
   const int64_t per = 16 / t.element_size();
-  return t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) % per == 0) && (t.size(0) == 1 || t.stride(0) % per == 0) &&
+  return t.stride(2) == 1 && (t.size(1) == 1 || (t.stride(1) % per == 0 && t.stride(1) <= 1 << 22)) && (t.size(0) == 1 || t.stride(0) % per == 0) &&
          reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
 }
 Tensor with_rows(const Tensor& t) { return t.numel() == 0 || rows_fit(t) ? t : dense(t); }

@@ -275,6 +275,23 @@ def test_nothing_reaches_an_earlier_frame(d, dv, at, poison, dtype):
         assert torch.equal(a[1, after], r[1, after]), name
 
 
+def test_rows_far_apart():
+    """A transposed view whose frames lie 2^22 elements and more apart is copied, not refused."""
+    from asr_amd.decay import decay_attention, decay_attention_train
+
+    dev = _dev()
+    q, k, v, w, _ = (t.to(dev) for t in _make(2, 3, 2, 32, 32, torch.bfloat16, 8))
+    ld = _decays(2).to(dev)
+    far = torch.empty(3 * ((1 << 22) + 64), dtype=torch.bfloat16, device=dev).as_strided((2, 3, 64), (64, (1 << 22) + 64, 1))
+    far.copy_(k)
+    assert torch.equal(decay_attention(q, far, v, 2, ld), decay_attention(q, k, v, 2, ld))
+    leaves = [q.clone().requires_grad_(True), far.detach().requires_grad_(True), v.clone().requires_grad_(True)]
+    got = torch.autograd.grad(decay_attention_train(*leaves, 2, ld), leaves, w)
+    leaves[1] = k.clone().requires_grad_(True)
+    ref = torch.autograd.grad(decay_attention_train(*leaves, 2, ld), leaves, w)
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
 def test_lengths_of_64_bits():
     from asr_amd.decay import decay_attention
 

@@ -104,14 +104,17 @@ int decay_launch_join(const DecayArgs& a, int roles, int state_elements, hipStre
   return e == hipSuccess ? 0 : set_error("launch of k_decay_join failed: %s", hipGetErrorString(e));
 }
 
+// Workgroups from which on they take the utterances from the longest to the shortest (up to 64 of them, those a wave can rank)
+constexpr long kDecayOrderFrom = 256;
+
 static bool decay_width(int d) { return d == 32 || d == 64 || d == 128; }
 
 static int decay_check(const char* what, int dtype, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv) {
   if (dtype != LMUFFT_F32 && dtype != LMUFFT_BF16) return set_error("%s: unknown dtype %d", what, dtype);
   if (B < 0 || T < 0 || H <= 0) return set_error("%s: bad shape (B=%d T=%d H=%d)", what, B, T, H);
   if (!decay_width(dk) || !decay_width(dv)) return set_error("%s: head widths %d, %d (supported: 32, 64, 128)", what, dk, dv);
-  // (HIP counts a launch's threads in 32 bits, 512 for each head; and the kernels an utterance's 16-byte pieces)
-  if ((long)B * H >= (1 << 23) || T > (1 << 25)) return set_error("%s: too large (B=%d T=%d H=%d)", what, B, T, H);
+  // (HIP counts a launch's threads in 32 bits, 512 for each head and role; and the kernels an utterance's 16-byte pieces)
+  if ((long)B * H > (1 << 21) || T > (1 << 25)) return set_error("%s: too large (B=%d T=%d H=%d)", what, B, T, H);
   return 0;
 }
 
@@ -146,7 +149,9 @@ static int decay_tensor(const char* what, const char* name, const void* p, int d
   return 0;
 }
 
-static int decay_launch_any(int dtype, const DecayArgs& a, int roles, int dk, int dv, hipStream_t st) {
+static int decay_launch_any(int dtype, DecayArgs a, int roles, int dk, int dv, hipStream_t st) {
+  a.roles = roles;
+  a.order = a.lengths && a.B > 1 && a.B <= 64 && (long)a.B * a.H * roles * a.segments > kDecayOrderFrom;
   return dtype == LMUFFT_BF16 ? decay_launch_bf16(a, roles, dk, dv, st) : decay_launch_f32(a, roles, dk, dv, st);
 }
 

@@ -66,7 +66,8 @@ struct DecayArgs {
   const int* lengths;      // [B] or NULL
   float* state;            // [B][H][DK][DV]: read at the start, replaced at the end; or NULL
   float scale;
-  int B, T, H, segments, seg_len, joined;
+  int B, T, H, segments, seg_len, joined, roles;
+  int order;  // workgroups take the utterances from the longest to the shortest
 };
 
 int decay_chunk_bf16(int dk, int dv);  // frames per chunk
@@ -192,6 +193,19 @@ __device__ __forceinline__ void dec_split(const dec_b8& v, const float w[8], dec
   }
 }
 
+// Which of up to 64 utterances is the rank-th longest (equal ones in their order), n: this lane's length, zero and more.  A
+// selection bit by bit from the highest: `left` are the utterances that share the bits so far with the one looked for.
+__device__ __forceinline__ int dec_ranked(int n, unsigned long long left, int rank, int most) {
+  for (int bit = 31 - __builtin_clz(most | 1); bit >= 0; --bit) {
+    const unsigned long long one = __ballot((n >> bit) & 1) & left;
+    const int c = __popcll(one);
+    left = rank < c ? one : left & ~one;
+    rank -= rank < c ? 0 : c;
+  }
+  const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(left >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)left, 0));
+  return __ffsll((unsigned long long)__ballot(before == rank) & left) - 1;
+}
+
 // Geometry of the kernels for one (type, DK, DV).
 template <class T, int DK, int DV>
 struct DecGeo {
@@ -229,13 +243,22 @@ __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k
   const DecTile<T, DK> qtile{vtile.base + C * DV};            // [C][DK]
   const DecTile<T, DK> stile{qtile.base + C * DK};            // [DV][DK]: S^T
 
-  const DecayRole& R = args.role[blockIdx.z];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;             // among those of its kind
   const bool holds = !OUT || __builtin_amdgcn_readfirstlane(tid >> 8) != 0;  // a wave of the state
-  const int bh = blockIdx.x, b = bh / args.H, h = bh - b * args.H, seg = blockIdx.y;
+  const int unit = blockIdx.x / args.H, h = blockIdx.x - unit * args.H, seg = blockIdx.y;
+  int b = unit / args.roles;
+  const DecayRole& R = args.role[unit - b * args.roles];
   const int T_ = args.T;
-  const int len = args.lengths ? min(max(args.lengths[b], 0), T_) : T_;
+  int len = T_;
+  if (args.order) {  // (every wave for itself)
+    const int n = lane < args.B ? min(max(args.lengths[lane], 0), T_) : 0;
+    b = dec_ranked(n, ~0ull >> (64 - args.B), b, T_);
+    len = __builtin_amdgcn_readlane(n, b);
+  } else if (args.lengths) {
+    len = min(max(args.lengths[b], 0), T_);
+  }
+  const int bh = b * args.H + h;
   const int s0 = seg * args.seg_len, s1 = min(s0 + args.seg_len, T_);
   const int end = min(s1, len);  // frames s0..end-1 are computed, end..s1-1 (of the padding) get zeros
   const bool first = s0 == 0, single = args.segments == 1;
@@ -555,13 +578,13 @@ static int decay_launch_terms(const DecayArgs& a, int roles, hipStream_t st) {
   }
   if (a.segments > 1) {
     ProfScope ps("k_decay_states", st);
-    hipLaunchKernelGGL((k_decay<T, DK, DV, false, TERMS>), dim3(a.B * a.H, a.segments - 1, roles), dim3(256),
+    hipLaunchKernelGGL((k_decay<T, DK, DV, false, TERMS>), dim3(a.B * a.H * a.roles, a.segments - 1), dim3(256),
                        G::kLdsState, st, a);
     if (a.joined && decay_launch_join(a, roles, DK * DV, st)) return 1;
   }
   {
     ProfScope ps("k_decay", st);
-    hipLaunchKernelGGL((k_decay<T, DK, DV, true, TERMS>), dim3(a.B * a.H, a.segments, roles), dim3(512), G::kLdsOut,
+    hipLaunchKernelGGL((k_decay<T, DK, DV, true, TERMS>), dim3(a.B * a.H * a.roles, a.segments), dim3(512), G::kLdsOut,
                        st, a);
   }
   const hipError_t e = hipGetLastError();

@@ -463,7 +463,7 @@ int lmufft_dropout_epoch(const uint32_t* epoch_dev);
  * q, k [B][T][H * dk], v, out [B][T][H * dv], all f32 or all bf16; ld* / bs* are the element strides of a frame and of an
  * utterance (rows start on 16-byte boundaries; a column block of a wider tensor is fine, inputs may repeat rows with stride
  * 0).  lengths [B] (or NULL) is clamped to [0, T]: frames behind it are not read, their outputs and gradients are zeros.
- * dk, dv in {32, 64, 128}; B * H < 2^23, T <= 2^25.  Sums and states are held in f32, added in a fixed order.  An infinity
+ * dk, dv in {32, 64, 128}; B * H <= 2^21, T <= 2^25.  Sums and states are held in f32, added in a fixed order.  An infinity
  * or a NaN inside a length reaches the frames from its own on (an infinity may come out as a NaN there), none before.
  *   lmufft_decay_attention: state [B][H][dk][dv] f32 (or NULL: zeros, and nothing is kept) is read as the state before
  *   the first frame and replaced by the state behind the last frame inside the length.

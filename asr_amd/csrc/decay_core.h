@@ -246,9 +246,14 @@ __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;             // among those of its kind
   const bool holds = !OUT || __builtin_amdgcn_readfirstlane(tid >> 8) != 0;  // a wave of the state
-  const int unit = blockIdx.x / args.H, h = blockIdx.x - unit * args.H, seg = blockIdx.y;
-  int b = unit / args.roles;
-  const DecayRole& R = args.role[unit - b * args.roles];
+  // Eight heads of one role, then the same eight of the next: workgroups go round the eight XCDs, so a head's roles meet in one
+  // XCD's L2, where two of them read the same rows of two tensors at about the same time.
+  const unsigned group = blockIdx.x / (8u * args.roles), place = blockIdx.x - group * (8u * args.roles);
+  const unsigned wide = min(8u, (unsigned)(args.B * args.H) - group * 8), role = place / wide;
+  const int ranked = group * 8 + (place - role * wide), seg = blockIdx.y;
+  int b = ranked / args.H;
+  const int h = ranked - b * args.H;
+  const DecayRole& R = args.role[role];
   const int T_ = args.T;
   int len = T_;
   if (args.order) {  // (every wave for itself)

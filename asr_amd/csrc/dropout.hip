@@ -1,7 +1,8 @@
 // Residual dropout on gfx950: out = res + keep x / (1 - p), the keep decisions recomputed from the element's place and the
 // call's two seeds (HashDropout, lmufft_internal.h), nothing stored.  The backward is the same kernel on the output's
 // gradient without a residual.  A thread takes eight neighbouring elements (16 bytes of bf16): one hash serves two of them.
-// HBM-bound: reads x and res once, writes out once.
+// HBM-bound: reads x and res once, writes out once (25600 x 384 bf16 onto f32: 19 us, 5.2 TB/s; its backward to bf16 12.5 us,
+// 4.7 TB/s).
 //
 // Rows of an even width below 2^32 pairs in all: a pair's hash index is its place in the whole tensor, no division.  Else
 // the row and column of a thread's first element come from one division and the others are counted on.

@@ -18,7 +18,10 @@
 //     k_gn_apply joins them and normalises, reading x again.  The backward does the same
 //     with the per-channel sums of dz and dz xhat, from which the group sums and the parameter gradients both follow.
 // Second moments are taken about a value of the data, never as a difference of large sums.  The utterances' statistics are
-// summed in 64 bits, everything else in 32.  Fixed order, no atomics.  HBM-bound.
+// summed in 64 bits, everything else in 32.  Fixed order, no atomics.  HBM-bound: 25600 rows x 384 in 6 groups bf16 10 us
+// (3.9 TB/s); 64 x 400 x 384 in 32 groups bf16 in columns 13.4 us, backward 23.8 + 4.2 us; 32 x 2999 x 384 in 8 groups f32 in
+// splits: statistics 28 us, result 45 us, backward 35 + 9 + 53 us, 780 MB in all at 4.6 TB/s, a large copy's rate (lengths from
+// a tenth of the frames up: about half of the frames are read, all are written).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

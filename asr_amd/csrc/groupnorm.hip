@@ -400,7 +400,8 @@ __device__ __forceinline__ void gn_join_groups(double s, double ss, int TR, int 
   }
 }
 
-// Workgroup (split, n) of the statistics over several workgroups: each split's sums of each group, part[n][split][G].
+// Workgroup (split, n) of the statistics over several workgroups: each split's sums of each group, part[n][split][G], and the
+// pivots behind them, [n][G]: k_gn_apply may write over x, whose first frame they come from.
 template <bool XB, int V>
 __global__ __launch_bounds__(1024) void k_gn_stats(GnArgs a) {
   __shared__ double2 red[1024];
@@ -420,6 +421,9 @@ __global__ __launch_bounds__(1024) void k_gn_stats(GnArgs a) {
   }
   double2* const out = reinterpret_cast<double2*>(a.part) + (n * a.splits + blockIdx.x) * a.G;
   gn_join_groups(s, ss, TR, RB, L, a.G, red, [&](int g, double u, double v) { out[g] = make_double2(u, v); });
+  double* const pivots = reinterpret_cast<double*>(reinterpret_cast<double2*>(a.part) + a.N * a.splits * a.G) + n * a.G;
+  if (blockIdx.x == 0)
+    for (int g = threadIdx.x; g < a.G; g += blockDim.x) pivots[g] = t1 > 0 ? gn_load<XB, 1>(a.x, base + g * cg).f[0] : 0.f;
 }
 
 template <bool XB, bool OB, int V>
@@ -429,6 +433,7 @@ __global__ __launch_bounds__(1024) void k_gn_apply(GnArgs a) {
   const int slot = threadIdx.x / TR, c = (threadIdx.x % TR) * V;
   const long n = blockIdx.y;
   const int len = gn_len(a, n);
+  const double* const pivots = reinterpret_cast<const double*>(reinterpret_cast<const double2*>(a.part) + a.N * a.splits * a.G) + n * a.G;
   // a group's splits are summed by a team of lanes (one thread a group took 0.8 us a split)
   int lanes = 1;
   while (lanes < 64 && lanes < a.splits) lanes <<= 1;
@@ -446,7 +451,7 @@ __global__ __launch_bounds__(1024) void k_gn_apply(GnArgs a) {
       ss += __shfl_xor(ss, o);
     }
     if (g < a.G && lane == 0) {
-      st[g] = gn_mean_rstd((double)len * cg, len > 0 ? gn_load<XB, 1>(a.x, n * a.T * a.C + g * cg).f[0] : 0.f, s, ss, a.eps);
+      st[g] = gn_mean_rstd((double)len * cg, (float)pivots[g], s, ss, a.eps);
       if (a.stats && blockIdx.x == 0) a.stats[n * a.G + g] = st[g];
     }
   }
@@ -785,7 +790,7 @@ static bool gn_plan(int64_t N, int32_t T, int32_t C, int32_t G, bool wide, bool 
 static size_t gn_workspace(const GnPlan& p, int64_t N, int32_t C, int32_t G, bool backward) {
   if (p.kind == kGnRows) return backward ? sizeof(float) * 2 * C * (size_t)p.blocks : 0;
   if (p.kind == kGnColumn) return backward ? sizeof(float) * 2 * C * (size_t)N : 0;
-  return backward ? sizeof(float) * 2 * ((size_t)N * p.splits * C + (size_t)N * G) : sizeof(double2) * (size_t)N * p.splits * G;
+  return backward ? sizeof(float) * 2 * ((size_t)N * p.splits * C + (size_t)N * G) : (sizeof(double2) * p.splits + sizeof(double)) * (size_t)N * G;
 }
 static dim3 gn_column_grid(const GnPlan& p, int64_t N) { return dim3((unsigned)((N + 7) / 8 * 8 * p.splits)); }
 

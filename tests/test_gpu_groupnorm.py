@@ -266,6 +266,28 @@ def test_captured_training_pass_replays():
             assert torch.equal(a, r), i
 
 
+@pytest.mark.parametrize("shape,groups", [((3, 2999, 384), 8), ((2, 5000, 96), 3), ((4, 100, 96), 4), ((500, 1, 384), 6)])
+def test_in_place(shape, groups):
+    """out == x of one dtype: what the result is made of is read before anything is written over it."""
+    from asr_amd import _lib
+    from asr_amd.groupnorm import group_norm
+
+    dev = _dev()
+    N, T, C = shape
+    x, w, b, _ = (t.to(dev) for t in _make(shape, torch.float32, 12))
+    lengths = torch.tensor([T, T // 2, 0, 1][:N], dtype=torch.int32, device=dev) if T > 1 else None
+    ref = group_norm(x, groups, w, b, activation="silu", lengths=lengths)
+    n = _lib.lib.lmufft_group_norm_workspace_bytes(N, T, C, groups, 0)
+    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+    for _ in range(20):
+        y = x.clone()
+        rc = _lib.lib.lmufft_group_norm(y.data_ptr(), _lib.F32, w.data_ptr(), b.data_ptr(), None if lengths is None else lengths.data_ptr(),
+                                        N, T, C, groups, 1e-5, 2, y.data_ptr(), _lib.F32, None, ws.data_ptr(), n,
+                                        torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, _lib.lib.lmufft_last_error()
+        assert torch.equal(y, ref)
+
+
 def test_lengths_of_64_bits():
     from asr_amd.groupnorm import group_norm
 

@@ -799,6 +799,7 @@ static int gn_check(const char* what, int x_dtype, int other, int64_t N, int32_t
   if (!known(x_dtype) || !known(other)) return set_error("%s: unknown dtype", what);
   if (N < 0 || T < 0 || C <= 0 || G <= 0 || C % G) return set_error("%s: bad shape (N=%lld T=%d C=%d G=%d)", what, (long long)N, T, C, G);
   if (C > kGnMaxWidth) return set_error("%s: %d channels (at most %d)", what, C, kGnMaxWidth);
+  if (T > (1 << 30)) return set_error("%s: %d frames (at most 2^30)", what, T);  // (frames are counted in 32 bits, strides on top)
   if (act < 0 || act > 2) return set_error("%s: unknown activation %d", what, act);
   return 0;
 }

@@ -465,6 +465,7 @@ int lmufft_dropout_epoch(const uint32_t* epoch_dev);
  * 0).  lengths [B] (or NULL) is clamped to [0, T]: frames behind it are not read, their outputs and gradients are zeros.
  * dk, dv in {32, 64, 128}; B * H <= 2^21, T <= 2^25.  Sums and states are held in f32, added in a fixed order.  An infinity
  * or a NaN inside a length reaches the frames from its own on (an infinity may come out as a NaN there), none before.
+ * Outputs and gradients must not overlap the inputs.
  *   lmufft_decay_attention: state [B][H][dk][dv] f32 (or NULL: zeros, and nothing is kept) is read as the state before
  *   the first frame and replaced by the state behind the last frame inside the length.
  *   lmufft_decay_attention_bwd: gradients of q, k, v for a forward that started from zeros (the decays are constants).
@@ -494,7 +495,8 @@ int lmufft_decay_attention_step(const void* q, const void* k, const void* v, int
  * T = 1 one row; y = act((x - mean) / sqrt(var + eps) * gamma + beta) with mean and (biased) variance over the frames
  * inside the length and the C / G channels of a group.  act: 0 none, 1 ReLU, 2 SiLU.  lengths [N] (NULL: all T frames)
  * is clamped to [0, T]; frames behind it are not read, their outputs and gradients are zeros.
- * C at most 1024, gamma, beta f32 [C], tensors start on 16-byte boundaries; statistics and sums in f32, fixed order.
+ * C at most 1024, N at most 65535 (rows, T = 1 without lengths: any number), T at most 2^30, gamma, beta f32 [C], tensors
+ * start on 16-byte boundaries; an utterance's statistics in f64, other sums in f32, fixed order.
  *   lmufft_group_norm: out f32 or bf16; stats [N][G][2] f64 (mean, rstd; may be NULL; not written for T = 1 without lengths) is
  *   what the backward reads.  In place (out == x) is fine with one dtype.
  *   lmufft_group_norm_bwd: dx (dtype of x), dgamma, dbeta f32 [C] (zeros for an empty x).

@@ -72,7 +72,7 @@ def test_c_entry_points_refuse_before_any_launch():
     for call, text in ((dict(dt=3), b"dtype"), (dict(od=-1), b"dtype"), (dict(C=97), b"bad shape"), (dict(G=0), b"bad shape"),
                        (dict(N=-1), b"bad shape"), (dict(C=1028), b"at most"), (dict(act=3), b"activation"), (dict(x=None), b"NULL"),
                        (dict(out=None), b"NULL"), (dict(x=q), b"16-byte"), (dict(T=5000), b"workspace"), (dict(T=5000, ws=p, n=8), b"workspace"),
-                       (dict(N=70000), b"utterances")):
+                       (dict(N=70000), b"utterances"), (dict(N=1, T=(1 << 30) + 1, C=1, G=1), b"frames")):
         assert fwd(**call) != 0 and text in lib.lmufft_last_error(), (call, lib.lmufft_last_error())
     assert fwd(N=0) == 0 and fwd(T=0) == 0
     assert lib.lmufft_group_norm_workspace_bytes(2, 5, 96, 5, 0) == 0

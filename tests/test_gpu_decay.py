@@ -275,6 +275,27 @@ def test_nothing_reaches_an_earlier_frame(d, dv, at, poison, dtype):
         assert torch.equal(a[1, after], r[1, after]), name
 
 
+@pytest.mark.parametrize("T,H,d,dv", [(1, 2, 64, 64), (3, 12, 64, 64), (17, 2, 32, 128), (32, 3, 128, 128), (64, 1, 64, 32)])
+def test_few_frames_lose_only_the_outputs_rounding(T, H, d, dv):
+    """Calls of one chunk in bf16: P in two bf16 terms (2^-9 each, 2^-16 M with room), the rest as in 32 bits, and half a step of
+    the result."""
+    from asr_amd.decay import decay_attention_train
+
+    dev = _dev()
+    q, k, v, w, _ = _make(2, T, H, d, dv, torch.bfloat16, 23)
+    w, ld = w.to(torch.bfloat16), _decays(H)
+    leaves = [t.to(dev).requires_grad_(True) for t in (q, k, v)]
+    out = decay_attention_train(*leaves, H, ld.to(dev))
+    got = [out.detach(), *torch.autograd.grad(out, leaves, w.to(dev))]
+    args = [t.double() for t in (q, k, v, w)]
+    size = [t.abs() for t in args]
+    ref = [do.decay_attention(*args[:3], ld.double())[0], *do.decay_attention_backward(*args, ld.double())]
+    M = [do.decay_attention(*size[:3], ld.double())[0], *do.decay_attention_backward(*size, ld.double())]
+    for name, g, r, m in zip(("out", "dq", "dk", "dv"), got, ref, M):
+        err = (g.double().cpu() - r).abs()
+        assert (err <= _bound32(m, T, max(d, dv)) + 2.0 ** -16 * m + 2.0 ** -8 * r.abs()).all(), (name, float(err.max()))
+
+
 def test_rows_far_apart():
     """A transposed view whose frames lie 2^22 elements and more apart is copied, not refused."""
     from asr_amd.decay import decay_attention, decay_attention_train

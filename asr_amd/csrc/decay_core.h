@@ -33,11 +33,11 @@
 // outputs 19); 16 x 400 x 6 f32 9 + 18 and 44 us: 13 chunks of 32 frames in the chain, 3.3 us each, 1.5 us of them the
 // exact-f32 products of one SIMD.
 //
-// Rounding: products accumulate in 32 bits and the state is held in 32 bits.  bf16 tensors: P and the copy of S that
-// multiplies q are rounded to bf16 once (what a bf16 operand of the matrix cores costs; each is below the rounding of the
-// output, and over many frames they average out; where one chunk is all there is, P keeps 16 bits in two terms -- a frame's
-// output may hang on one P, and the launch takes the time anyway); the scaled v that enters the state is split into bf16 terms,
-// three where the state is returned (24 bits are kept).
+// Rounding: products accumulate in 32 bits and the state is held in 32 bits.  bf16 tensors: P enters its product in two bf16
+// terms (2^-16 of a P is lost: an output may hang on a single one, at the start of an utterance or under a fast decay, and one
+// term would cost it as much as the rounding of the result; one term 16.9 us forward and 34.1 backward at 64 x 400 x 6, two 17.7
+// and 36.4); the copy of S that multiplies q is rounded to bf16 once; the scaled
+// v that enters the state is split into two terms, three where the state is returned (24 bits are kept).
 // f32 tensors: the exact-f32 matrix instruction throughout.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -119,13 +119,10 @@ __device__ __forceinline__ void dec_pack(DecTraits<float>::frag& f, const dec_f4
   f.a = lo;
   f.b = hi;
 }
-// what dec_pack's rounding leaves of lo, hi (nothing of an infinity)
+// what dec_pack's rounding leaves of lo, hi (a NaN of an infinity)
 __device__ __forceinline__ void dec_rest(dec_b8& f, const dec_b8& packed, const dec_f4& lo, const dec_f4& hi) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float a = lo[e] - (float)packed[e], b = hi[e] - (float)packed[4 + e];
-    f[e] = (__bf16)(__builtin_isfinite(a) ? a : 0.f), f[4 + e] = (__bf16)(__builtin_isfinite(b) ? b : 0.f);
-  }
+  for (int e = 0; e < 4; ++e) f[e] = (__bf16)(lo[e] - (float)packed[e]), f[4 + e] = (__bf16)(hi[e] - (float)packed[4 + e]);
 }
 __device__ __forceinline__ void dec_store4(__bf16* p, const dec_f4& v) {
   dec_b4 o;
@@ -243,8 +240,7 @@ struct DecGeo {
 // states at the ends of all segments but the last (which the OUT kernel joins), from zero or, in the first segment, from the
 // initial state.
 // TERMS: bf16 terms of the scaled v that enters the state (see above): three where the state is returned, two where it only
-// serves outputs that are rounded to bf16 themselves.  Calls of one chunk take the form with three, which also has the second
-// term of P (a test for it in the other form cost 3 % of every call).
+// serves outputs that are rounded to bf16 themselves.
 template <class T, int DK, int DV, bool OUT, int TERMS>
 __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k_decay(DecayArgs args) {
   typedef DecGeo<T, DK, DV> G;
@@ -440,16 +436,17 @@ __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k
           }
           Frag pf;
           dec_pack(pf, p[0], p[1]);
-          if constexpr (sizeof(T) == 2 && TERMS == 3) {
-            if (T_ <= C) {  // one chunk in all: what the rounding of P leaves
-              Frag low;
-              dec_rest(low, pf, p[0], p[1]);
+          if constexpr (sizeof(T) == 2) {
+            Frag low, vx[MO];
+            dec_rest(low, pf, p[0], p[1]);
 #pragma unroll
-              for (int i = 0; i < MO; ++i) o[i] = dec_mma(vtile.col_frag(32 * jb, 16 * (mo0 + i), l16, g), low, o[i]);
-            }
+            for (int i = 0; i < MO; ++i) o[i] = dec_mma(vx[i] = vtile.col_frag(32 * jb, 16 * (mo0 + i), l16, g), low, o[i]);
+#pragma unroll
+            for (int i = 0; i < MO; ++i) o[i] = dec_mma(vx[i], pf, o[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < MO; ++i) o[i] = dec_mma(vtile.col_frag(32 * jb, 16 * (mo0 + i), l16, g), pf, o[i]);
           }
-#pragma unroll
-          for (int i = 0; i < MO; ++i) o[i] = dec_mma(vtile.col_frag(32 * jb, 16 * (mo0 + i), l16, g), pf, o[i]);
         }
         dec_f4 odd = dec_f4(0.f);
 #pragma unroll
@@ -626,8 +623,7 @@ static int decay_launch_terms(const DecayArgs& a, int roles, hipStream_t st) {
 template <class T, int DK, int DV>
 static int decay_launch(const DecayArgs& a, int roles, hipStream_t st) {
   if constexpr (sizeof(T) == 4) return decay_launch_terms<T, DK, DV, 1>(a, roles, st);
-  else return a.state || a.T <= DecGeo<T, DK, DV>::C ? decay_launch_terms<T, DK, DV, 3>(a, roles, st)
-                                                     : decay_launch_terms<T, DK, DV, 2>(a, roles, st);
+  else return a.state ? decay_launch_terms<T, DK, DV, 3>(a, roles, st) : decay_launch_terms<T, DK, DV, 2>(a, roles, st);
 }
 
 #define DECAY_FOR_WIDTHS(T, DK_, DV_, RESULT, EXPR)                        \

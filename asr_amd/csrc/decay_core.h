@@ -33,11 +33,12 @@
 // outputs 19); 16 x 400 x 6 f32 9 + 18 and 44 us: 13 chunks of 32 frames in the chain, 3.3 us each, 1.5 us of them the
 // exact-f32 products of one SIMD.
 //
-// Rounding: products accumulate in 32 bits and the state is held in 32 bits.  bf16 tensors: P enters its product in two bf16
-// terms (2^-16 of a P is lost: an output may hang on a single one, at the start of an utterance or under a fast decay, and one
-// term would cost it as much as the rounding of the result; one term 16.9 us forward and 34.1 backward at 64 x 400 x 6, two 17.7
-// and 36.4); the copy of S that multiplies q is rounded to bf16 once; the scaled
-// v that enters the state is split into two terms, three where the state is returned (24 bits are kept).
+// Rounding: products accumulate in 32 bits and the state is held in 32 bits.  bf16 tensors: P and the copy of S that multiplies
+// q enter their products in two bf16 terms each, so 2^-16 of a value is lost: an output may hang on a single P, at the start of
+// an utterance or under a fast decay, or on the state alone, and one term would cost it as much as the rounding of the result
+// (0.0023 of the results' norm in error, 0.0017 with two).  Measured at 64 x 400 x 6: one term each 16.9 us forward and 34.1
+// backward, P in two 17.7 and 36.4, both 19.0 and 38.5; 32 x 3000 x 6 76 and 111, 81 and 114, 87 and 119.  The scaled v that
+// enters the state is split into two terms, three where the state is returned (24 bits are kept).
 // f32 tensors: the exact-f32 matrix instruction throughout.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -179,8 +180,8 @@ struct DecTile {
     }
     return f;
   }
-  // four elements of a row from a column that is a multiple of four
-  __device__ __forceinline__ void put4(int row, int c, const dec_f4& v) const { dec_store4(piece(row, c / VEC) + c % VEC, v); }
+  // where four elements of a row lie, from a column that is a multiple of four on
+  __device__ __forceinline__ T* four(int row, int c) const { return piece(row, c / VEC) + c % VEC; }
 };
 
 // lambda^n for n >= 0 from log2 lambda, which is held above -2^100 so that lambda = 0 gives lambda^0 = 1 (and 0 behind it)
@@ -232,7 +233,8 @@ struct DecGeo {
   static constexpr int KT = DK / 16 / KS;             // row tiles of a wave's part
   static constexpr int VEC = DecTraits<T>::kVec;
   static constexpr size_t kLdsState = sizeof(T) * (size_t)C * (DK + DV);
-  static constexpr size_t kLdsOut = kLdsState + sizeof(T) * (size_t)(C + DV) * DK;
+  static constexpr int STERMS = sizeof(T) == 2 ? 2 : 1;  // terms of the state's copy
+  static constexpr size_t kLdsOut = kLdsState + sizeof(T) * (size_t)(C + STERMS * DV) * DK;
   static constexpr int WAVES = kLdsOut <= 40 * 1024 && DV <= 64 ? 4 : 2;  // a SIMD: two workgroups of eight waves a CU, or one
 };
 
@@ -256,6 +258,7 @@ __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k
   const DecTile<T, DV> vtile{ktile.base + C * DK};            // [C][DV]
   const DecTile<T, DK> qtile{vtile.base + C * DV};            // [C][DK]
   const DecTile<T, DK> stile{qtile.base + C * DK};            // [DV][DK]: S^T
+  const DecTile<T, DK> srest{stile.base + DV * DK};           // bf16: what its rounding left
 
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;             // among those of its kind
@@ -409,12 +412,16 @@ __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k
       dec_f4 o[MO];
       for (bool again = false;; again = true) {
 #pragma unroll
-        for (int i = 0; i < MO; ++i) {
-          o[i] = dec_f4(0.f);
+        for (int i = 0; i < MO; ++i) o[i] = dec_f4(0.f);
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) o[i] = dec_mma(stile.row_frag(16 * (mo0 + i) + l16, kb, g), qx[kb], o[i]);
-          o[i] *= fq;
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+          for (int i = 0; i < (G::STERMS == 2 ? MO : 0); ++i) o[i] = dec_mma(srest.row_frag(16 * (mo0 + i) + l16, kb, g), qx[kb], o[i]);
+#pragma unroll
+          for (int i = 0; i < MO; ++i) o[i] = dec_mma(stile.row_frag(16 * (mo0 + i) + l16, kb, g), qx[kb], o[i]);
         }
+#pragma unroll
+        for (int i = 0; i < MO; ++i) o[i] *= fq;
 #pragma unroll 1
         for (int jb = 0; jb <= it >> 1; ++jb) {
           dec_f4 p[2];
@@ -513,13 +520,33 @@ __global__ __launch_bounds__(OUT ? 512 : 256, (DecGeo<T, DK, DV>::WAVES)) void k
     for (int r = 0; r < 4; ++r) wend[r] = dec_pow(a2, 15 - (4 * g + r));
     for (int t0 = s0; t0 < end; t0 += C) {
       const int n = min(C, end - t0);  // frames of this chunk
+      // the state's copy, rounded before the barrier (between the two there is only its way to LDS)
+      constexpr bool TWO = OUT && G::STERMS == 2;
+      dec_b4 copy[TWO ? KT : 1][MS], rest[TWO ? KT : 1][MS];
+      if constexpr (TWO) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int m = 0; m < MS; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              copy[t][m][r] = (__bf16)S[t][m][r];
+              rest[t][m][r] = (__bf16)(S[t][m][r] - (float)copy[t][m][r]);
+            }
+      }
       begin(t0, [&] {
-        if (OUT) {
 #pragma unroll
-          for (int t = 0; t < KT; ++t)
+        for (int t = 0; t < (OUT ? KT : 0); ++t)
 #pragma unroll
-            for (int m = 0; m < MS; ++m) stile.put4(scol + 16 * m + l16, srow + 16 * t + 4 * g, S[t][m]);
-        }
+          for (int m = 0; m < MS; ++m) {
+            const int row = scol + 16 * m + l16, c = srow + 16 * t + 4 * g;
+            if constexpr (TWO) {
+              *reinterpret_cast<dec_b4*>(stile.four(row, c)) = copy[t][m];
+              *reinterpret_cast<dec_b4*>(srest.four(row, c)) = rest[t][m];
+            } else {
+              dec_store4(stile.four(row, c), S[t][m]);
+            }
+          }
       });
       const float lam = upow(n);
 #pragma unroll

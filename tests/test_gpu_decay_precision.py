@@ -1,9 +1,10 @@
-"""GPU tests of what the bf16 decay attention rounds before its result: a score loses nothing above sixteen bits, whatever the
-length of the call or the batch around an utterance.
+"""GPU tests of what the bf16 decay attention rounds before its result: nothing below sixteen bits, whatever the length of the
+call, the batch around an utterance, or the place of a frame.
 
-Tolerance.  A bf16 keeps 2^-8 of a value at worst, two of them 2^-16, so a score in two terms loses 2^-16 M, M the sum of the
-magnitudes of an output's terms; 2^-15 M is allowed, besides the 32-bit bound of tests/test_gpu_decay.py and half a step of the
-result, 2^-8 |ref|."""
+Tolerance.  A bf16 keeps 2^-8 of a value at worst, two of them 2^-16.  A term of an output passes through one score (two bf16
+terms), or through the state: the scaled v that enters it and the state's copy that multiplies q, two terms each; so 2^-15 M
+in all, M the sum of the terms' magnitudes; besides the 32-bit bound of tests/test_gpu_decay.py and half a step of the result,
+2^-8 |ref|."""
 import pytest
 import torch
 
@@ -51,3 +52,40 @@ def test_an_utterance_alone_and_in_a_padded_batch(H, d, dv):
         size = [t.abs() for t in part]
         for name, got, r, m in zip(("out", "dq", "dk", "dv"), alone, _refs(*part, ld, None), _refs(*size, ld, None)):
             _tight(name, got, r, m, n, max(d, dv))
+
+
+SHAPES = [
+    # B, T, H, dk, dv, lengths
+    (3, 200, 5, 64, 64, [200, 3, 70]),
+    (2, 129, 2, 32, 128, None),
+    (2, 150, 3, 128, 128, [150, 65]),
+    (2, 333, 2, 128, 32, [333, 64]),
+    (1, 1001, 5, 64, 64, None),         # several segments
+    (1, 4000, 2, 32, 64, [3911]),       # joined by a launch of their own
+]
+
+
+@pytest.mark.parametrize("B,T,H,dk,dv,lengths", SHAPES)
+def test_every_frame_without_a_state(B, T, H, dk, dv, lengths):
+    q, k, v, w, _ = _make(B, T, H, dk, dv, torch.bfloat16, T)
+    w, ld = w.to(torch.bfloat16), _decays(H)
+    got = _call(q, k, v, w, H, ld, lengths)
+    size = [t.abs() for t in (q, k, v, w)]
+    for name, g, r, m in zip(("out", "dq", "dk", "dv"), got, _refs(q, k, v, w, ld, lengths), _refs(*size, ld, lengths)):
+        _tight(name, g, r, m, T, max(dk, dv))
+
+
+@pytest.mark.parametrize("B,T,H,dk,dv,lengths", SHAPES + [(4, 1, 6, 64, 64, None), (3, 50, 6, 64, 64, [50, 0, 7])])
+def test_every_frame_from_a_state(B, T, H, dk, dv, lengths):
+    from asr_amd.decay import decay_attention
+
+    dev = _dev()
+    q, k, v, _, st = _make(B, T, H, dk, dv, torch.bfloat16, T + 1)
+    ld = _decays(H)
+    ln = None if lengths is None else torch.tensor(lengths, device=dev)
+    sd = st.to(dev)
+    out = decay_attention(*(t.to(dev) for t in (q, k, v)), H, ld.to(dev), ln, sd)
+    ref, S = do.decay_attention(q, k, v, ld, lengths, st)
+    M, MS = do.decay_attention(q.abs(), k.abs(), v.abs(), ld, lengths, st.abs())
+    _tight("out", out, ref, M, T, dk)
+    assert ((sd.double().cpu() - S).abs() <= _bound32(MS, T, 0)).all()

@@ -804,6 +804,15 @@ static int gn_check(const char* what, int x_dtype, int other, int64_t N, int32_t
   return 0;
 }
 static bool gn_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// A result over an input is fine where every thread overwrites exactly what it has read: the same place and the same dtype.
+static int gn_check_alias(const char* what, const char* out_name, const void* out, int out_dtype, const char* in_name,
+                          const void* in, int in_dtype, int64_t rows, int32_t C) {
+  auto bytes = [&](int dtype) { return (unsigned __int128)rows * (unsigned)C * (dtype == LMUFFT_F32 ? 4 : 2); };
+  const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(in);
+  const bool apart = o + bytes(out_dtype) <= i || i + bytes(in_dtype) <= o;
+  if (apart || (o == i && out_dtype == in_dtype)) return 0;
+  return set_error("%s: %s may alias %s only at its start and with the same dtype", what, out_name, in_name);
+}
 
 #define GN_BY_V4(V_, CALL)                           \
   do {                                               \
@@ -855,6 +864,7 @@ extern "C" int lmufft_group_norm(const void* x, int x_dtype, const float* gamma,
   if (!rows && N > 65535) return set_error("%s: %lld utterances (at most 65535)", what, (long long)N);
   if (!gn_aligned(x) || !gn_aligned(gamma) || !gn_aligned(beta) || !gn_aligned(out) || !gn_aligned(stats))
     return set_error("%s: tensors must start on 16-byte boundaries", what);
+  if (gn_check_alias(what, "out", out, out_dtype, "x", x, x_dtype, N * T, C)) return 1;
   GnPlan p;
   const bool xb = x_dtype == LMUFFT_BF16, ob = out_dtype == LMUFFT_BF16;
   if (!gn_plan(N, T, C, G, xb && ob, rows, false, xb ? 2 : 4, &p)) return set_error("%s: %d channels in %d groups", what, C, G);
@@ -906,6 +916,9 @@ extern "C" int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy,
   if (!gn_aligned(x) || !gn_aligned(dy) || !gn_aligned(gamma) || !gn_aligned(beta) || !gn_aligned(dx) ||
       !gn_aligned(stats))
     return set_error("%s: tensors must start on 16-byte boundaries", what);
+  if (gn_check_alias(what, "dx", dx, x_dtype, "x", x, x_dtype, N * T, C) ||
+      gn_check_alias(what, "dx", dx, x_dtype, "dy", dy, dy_dtype, N * T, C))
+    return 1;
   GnPlan p;
   const bool xb = x_dtype == LMUFFT_BF16, gb = dy_dtype == LMUFFT_BF16;
   if (!gn_plan(N, T, C, G, xb && gb, rows, true, xb ? 2 : 4, &p))

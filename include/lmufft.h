@@ -498,8 +498,9 @@ int lmufft_decay_attention_step(const void* q, const void* k, const void* v, int
  * C at most 1024, N at most 65535 (rows, T = 1 without lengths: any number), T at most 2^30, gamma, beta f32 [C], tensors
  * start on 16-byte boundaries; an utterance's statistics in f64, other sums in f32, fixed order.
  *   lmufft_group_norm: out f32 or bf16; stats [N][G][2] f64 (mean, rstd; may be NULL; not written for T = 1 without lengths) is
- *   what the backward reads.  In place (out == x) is fine with one dtype.
- *   lmufft_group_norm_bwd: dx (dtype of x), dgamma, dbeta f32 [C] (zeros for an empty x).
+ *   what the backward reads.  In place (out == x) is fine with one dtype; any other overlap of the two is refused.
+ *   lmufft_group_norm_bwd: dx (dtype of x), dgamma, dbeta f32 [C] (zeros for an empty x).  dx may be x, or dy of the same
+ *   dtype; any other overlap with them is refused.
  * ---------------------------------------------------------------------- */
 size_t lmufft_group_norm_workspace_bytes(int64_t N, int32_t T, int32_t C, int32_t G, int backward);
 int lmufft_group_norm(const void* x, int x_dtype, const float* gamma, const float* beta, const int32_t* lengths,

@@ -76,3 +76,37 @@ def test_under_autocast():
 ])
 def test_more_rows_than_workgroups(shape, groups, activation, dtype):
     _check(shape, groups, None, activation, dtype, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,groups", [((700, 384), 6), ((9, 1000), 8), ((3, 400, 384), 32), ((2, 2999, 384), 8)])
+def test_the_backward_in_place(shape, groups, dtype):
+    """dx over x, and over dy of the same dtype."""
+    from asr_amd import _lib
+    from asr_amd.groupnorm import group_norm_train
+
+    dev = _dev()
+    x, w, b, dy = (t.to(dev) for t in _make(shape, dtype, 3))
+    dy = dy.to(dtype)
+    N, T, C = shape if len(shape) == 3 else (shape[0], 1, shape[1])
+    leaves = [x.clone().requires_grad_(True), w.clone().requires_grad_(True), b.clone().requires_grad_(True)]
+    ref = torch.autograd.grad(group_norm_train(leaves[0], groups, *leaves[1:], 1e-5, "silu"), leaves, dy)
+    code = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}[dtype]
+    n = _lib.lib.lmufft_group_norm_workspace_bytes(N, T, C, groups, 1)
+    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+    m = _lib.lib.lmufft_group_norm_workspace_bytes(N, T, C, groups, 0)
+    ws2 = torch.empty(max(m, 16), dtype=torch.uint8, device=dev)
+    stats = torch.empty(N, groups, 2, dtype=torch.float64, device=dev)
+    y = torch.empty_like(x)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert _lib.lib.lmufft_group_norm(x.data_ptr(), code, w.data_ptr(), b.data_ptr(), None, N, T, C, groups, 1e-5, 2, y.data_ptr(), code,
+                                      stats.data_ptr(), ws2.data_ptr(), m, stream) == 0, _lib.lib.lmufft_last_error()
+    for over in ("x", "dy"):
+        xx, dd = x.clone(), dy.clone()
+        dx = xx if over == "x" else dd
+        dw, db = torch.empty_like(w), torch.empty_like(b)
+        rc = _lib.lib.lmufft_group_norm_bwd(xx.data_ptr(), code, dd.data_ptr(), code, w.data_ptr(), b.data_ptr(), None, stats.data_ptr(),
+                                            N, T, C, groups, 1e-5, 2, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n, stream)
+        assert rc == 0, _lib.lib.lmufft_last_error()
+        for got, r in zip((dx, dw, db), ref):
+            assert torch.equal(got, r), over

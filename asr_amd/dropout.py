@@ -18,7 +18,6 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._call import ops
 
 _EPOCHS = {}  # device index -> int32 tensor [1], registered with the library for that device
 
@@ -63,6 +62,7 @@ def check_capturable(device, p_drop: float, seeds_given: bool) -> None:
 
 
 _dropout_calls = 0
+_ops = None  # the bound operators, loaded by the first dropout_add: what else is here needs the C library only
 
 
 def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, p_drop: float = 0.1, seeds=None,
@@ -74,7 +74,9 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, p_drop
     `seeds` = (seed0, seed1), two 32-bit integers that name the mask; by default torch's seed and a per-process call
     counter.  Under HIP graph capture the seeds are frozen and the device's epoch counter gives every replay its own mask
     (see above); without that counter such a capture raises."""
-    global _dropout_calls
+    global _dropout_calls, _ops
+    if _ops is None:
+        from ._call import ops as _ops
     if not 0.0 <= p_drop < 1.0:
         raise ValueError(f"dropout probability has to be in [0, 1), got {p_drop}")
     if seeds is None:
@@ -83,4 +85,4 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, p_drop
         if p_drop > 0:
             _dropout_calls += 1
         seeds = (torch.initial_seed() & 0xFFFFFFFF, 0x44520000 ^ (_dropout_calls & 0xFFFFFFFF))
-    return ops.dropout_add(x, residual, p_drop, int(seeds[0]) & 0xFFFFFFFF, int(seeds[1]) & 0xFFFFFFFF, out_dtype)
+    return _ops.dropout_add(x, residual, p_drop, int(seeds[0]) & 0xFFFFFFFF, int(seeds[1]) & 0xFFFFFFFF, out_dtype)

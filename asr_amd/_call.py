@@ -14,4 +14,8 @@ if not os.path.exists(os.path.join(os.path.dirname(os.path.abspath(__file__)), "
                       "(or `python -c 'import __graft_entry__ as g; g.build()'`). asr_amd has no CPU or eager fallback.")
 from . import _torch_ops as ops  # noqa: E402
 
+# the entry points are bound by name: only the version tells that their arguments are those the binding was compiled for
+if getattr(ops, "abi_version", None) != _lib.ABI_VERSION:
+    raise ImportError(f"asr_amd/_torch_ops.so: ABI version {getattr(ops, 'abi_version', None)}, expected {_lib.ABI_VERSION}; "
+                      "rebuild it (`make -C asr_amd/csrc`)")
 ops.bind({name: ctypes.cast(getattr(_lib.lib, name), ctypes.c_void_p).value for name in ops.entries if name})

@@ -478,6 +478,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("group_norm", &group_norm, free_gil());
   m.def("group_norm_train", &group_norm_train, free_gil());
   m.def("dropout_add", &dropout_add, free_gil());
+  m.attr("abi_version") = LMUFFT_ABI_VERSION;  // of the signatures compiled in
   m.attr("entries") = py::make_tuple(
 #define X(name) #name,
       LMUFFT_ENTRIES(X)

@@ -24,3 +24,29 @@ except ImportError:
 else:
     raise SystemExit("dropout_add ran without the binding")
 """)
+
+
+def test_a_binding_of_another_abi_is_refused():
+    _python("""
+import sys, types
+from asr_amd import _lib
+for version in (_lib.ABI_VERSION - 1, None):  # (a binding from before it carried its version)
+    stub = types.ModuleType("asr_amd._torch_ops")
+    stub.entries, stub.bind = ("",), lambda at: None
+    if version is not None:
+        stub.abi_version = version
+    sys.modules["asr_amd._torch_ops"] = stub
+    sys.modules.pop("asr_amd._call", None)
+    try:
+        import asr_amd._call
+    except ImportError as e:
+        assert "ABI version" in str(e), e
+    else:
+        raise SystemExit(f"a binding of ABI version {version} was bound")
+""")
+
+
+def test_the_binding_carries_the_library_s_abi_version():
+    from asr_amd import _call, _lib
+
+    assert _call.ops.abi_version == _lib.ABI_VERSION == _lib.lib.lmufft_abi_version()

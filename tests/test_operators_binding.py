@@ -1,7 +1,10 @@
-"""CPU-side checks of the operators' binding (asr_amd/_torch_ops.so)."""
+"""CPU-side checks of the operators' binding (asr_amd/_torch_ops.so) and of the build."""
 import os
+import shutil
 import subprocess
 import sys
+
+import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -50,3 +53,12 @@ def test_the_binding_carries_the_library_s_abi_version():
     from asr_amd import _call, _lib
 
     assert _call.ops.abi_version == _lib.ABI_VERSION == _lib.lib.lmufft_abi_version()
+
+
+@pytest.mark.skipif(shutil.which("make") is None, reason="needs make")
+def test_a_change_of_the_build_flags_rebuilds_every_object():
+    csrc = os.path.join(ROOT, "asr_amd", "csrc")
+    plan = subprocess.run(["make", "-C", csrc, "-n", "-W", os.path.join(csrc, "Makefile")], capture_output=True, text=True, check=True).stdout
+    for name in sorted(os.listdir(csrc)):
+        if name.endswith(".hip"):
+            assert f"build/{name[:-4]}.o " in plan, name

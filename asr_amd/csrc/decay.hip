@@ -60,7 +60,7 @@ __global__ __launch_bounds__(kDecayStepThreads) void k_decay_step(const T* __res
 
 // k_decay_join: a workgroup takes 64 places (16 bytes each) of one head's states, its sixteen waves up to eight consecutive
 // segments each, read at once.  A wave first sums its own, the waves' sums meet in LDS.  (Summed by every segment's workgroup for
-// itself instead, 62 segments of one head cost 24 us of reads.)  124 segments of six heads 64 x 64: 6.9 us, 24 MB there and back.
+// itself instead, 62 segments of one head cost 24 us of reads.)  74 segments of six heads 64 x 64: 5.4 us, 14 MB there and back.
 constexpr int kJoinEach = kDecayMaxSegments / 16;
 __global__ __launch_bounds__(1024) void k_decay_join(float* ws, long role_stride, const float* __restrict__ log_decay,
                                                      const int* __restrict__ lengths, int T, int H, int segments, int seg_len,
@@ -122,15 +122,24 @@ static int decay_check(const char* what, int dtype, int32_t B, int32_t T, int32_
   return 0;
 }
 
-// Segments an utterance's frames are split into when there are few heads in all: one workgroup walks a chunk in 1.5 us, and
-// about 200 of them saturate the memory.  A split costs a second read of k and v and a launch, from kDecayJoinFrom segments on
-// another one.  Measured, whole call: 6 heads of 23999 frames bf16 in 46 segments 42.6 us, in 124 37.7 us; 96 heads of 400 frames
-// f32 in 2 segments 31.1 us, in 3 27.9 us, in 5 34.0 us; 192 heads of 3000 frames bf16 whole 77 us, in 2 83 us, in 3 75 us; their
-// backward (576) whole 113 us, in 2 151 us; the backward of 96 heads of 400 frames f32 (288) whole 44 us, in 2 45 us.
+// Segments an utterance's frames are split into when there are few heads in all (counted over utterances and roles).  A split
+// costs a second read of k and v and a launch, from kDecayJoinFrom segments on another one, and pays while CUs are idle or the
+// longest utterance's chunks are what is waited for.  Heads of up to 64 columns leave a CU room for two workgroups, and long
+// utterances are split into about that many, 480; wider heads have a CU each, and short utterances are in so few chunks that the
+// launches weigh: 320.  Measured, whole call in us (all utterances full / lengths from a tenth up), by segments:
+//   480 or fewer  f32 96 heads of 3000 frames 5: 123 / 120, 3: 162 / 119; bf16 24 heads of 3000 16: 27 / 27, 12: 29 / 26; one
+//                 utterance of 24000 bf16 of 24 heads 20: 103, 13: 133, of 17 27: 74, 18: 97; 192 heads of 3000 bf16 2: 92 / 75,
+//                 whole: 85 / 84, 240 heads 2: 102 / 90, whole: 94 / 85; backward of 144 (3 x 48) heads of 3000 bf16 3: 68 / 63,
+//                 2: 88 / 69, of 288 whole: 122 / 86, 2: 128 / 89
+//   480 or more   one utterance of 24000 bf16 of 6 heads 75: 36, 125: 40, of 16 29: 69, 47: 70; of 8000 of 12 32: 30, 42: 28
+//   32 chunks     f32 96 heads of 1000 3: 62 / 47, 5: 58 / 56; 72 (3 x 24) heads' backward 4: 50 / 38, 6: 50 / 50; above (47 and
+//                 94 chunks) see the first lines
+//   128 columns   bf16 24 heads of 3000 12: 74 / 49, 16: 66 / 63, 10: 54 / 52; 96 heads 3: 184 / 113, 5: 157 / 148, 2: 160 / 159
 static int decay_segments(int dtype, int32_t B, int32_t T, int32_t H, int32_t dk, int32_t dv, int roles, int* seg_len) {
   const int chunk = dtype == LMUFFT_BF16 ? decay_chunk_bf16(dk, dv) : decay_chunk_f32(dk, dv);
   const long heads = std::max<long>(1, (long)B * H * roles), chunks = std::max<long>(1, (T + (long)chunk - 1) / chunk);
-  long n = std::min<long>((heads <= 16 ? 768 : 320) / heads, chunks / 2);  // (no segment of a single chunk)
+  const long workgroups = chunks > 32 && std::max(dk, dv) <= 64 ? 480 : 320;
+  long n = std::min<long>(workgroups / heads, chunks / 2);  // (no segment of a single chunk)
   n = std::max<long>(std::min<long>(n, kDecayMaxSegments), 1);
   const long per = (chunks + n - 1) / n;
   *seg_len = (int)(per * chunk);

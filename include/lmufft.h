@@ -514,9 +514,9 @@ int lmufft_group_norm_bwd(const void* x, int x_dtype, const void* dy, int dy_dty
 /* ------------------------------------------------------------------------
  * Residual dropout: out = res + keep x / (1 - p_drop) on rows of C elements (res may be NULL), the keep decisions by
  * the hash given at lmufft_attention_fwd_train with rows of C columns and the epoch of lmufft_dropout_epoch; no mask is
- * stored, and the backward is the same call on the gradient of `out` without `res`.  Replaces nn.Dropout where nothing in
- * front of it can take it along (src/models/lmu_encoder.py:232).  f32 or bf16 each, dense, 16-byte aligned; out may be x or
- * res of the same dtype.
+ * stored, and the backward is the same call on the gradient of `out` without `res`.  For an nn.Dropout that stands alone;
+ * the reference's (src/models/lmu_encoder.py:45, 86, 232) all stand beside a softmax or a layer norm and are fused with them
+ * above.  f32 or bf16 each, dense, 16-byte aligned; out may be x or res of the same dtype.
  * ---------------------------------------------------------------------- */
 int lmufft_dropout_add(const void* x, int x_dtype, const void* res, int res_dtype, int64_t rows, int32_t C,
                        float p_drop, uint32_t seed0, uint32_t seed1, void* out, int out_dtype, void* stream);

@@ -106,9 +106,10 @@ int decay_launch_join(const DecayArgs& a, int roles, int state_elements, hipStre
 }
 
 // Workgroups from which on they take the utterances from the longest to the shortest (up to 64 of them, those a wave can rank):
-// a CU's second workgroups are then the short ones, and none starts late.  Lengths from a tenth up: 64 x 400 x 6 heads bf16
-// 16.7 -> 15.2 us, 16 x 400 f32 with its backward 76.7 -> 66.2 us, the backward of 32 x 3000 bf16 119.7 -> 113.5 us.  With a
-// workgroup a CU or fewer the order changes nothing, and the ranking costs 0.3 us.
+// a CU's second workgroups are then the short ones, and none starts late.  Kernel times, lengths from a tenth up, in the batch's
+// order and in this one: 64 x 400 x 6 heads bf16 22.0 and 19.0 us, backward 42 and 38; backward of 16 x 400 f32 51 and 44; 32 x
+// 3000 bf16 66 and 57, backward 144 and 122.  With a workgroup a CU or fewer the order changes nothing, and the ranking costs
+// 0.3 us.  Batches above 64 keep their own order.
 constexpr long kDecayOrderFrom = 256;
 
 static bool decay_width(int d) { return d == 32 || d == 64 || d == 128; }

@@ -23,15 +23,16 @@
 //   S  += K^T (w V)      A = K^T columns, B = V^T columns scaled by lambda^(C-1-j)
 // q, k, v go through LDS by rows, as they lie in memory, and the state in the products' type; columns are read from there by
 // the transposing LDS read (bf16) or element by element (f32).  Rows are stored without padding, their 16-byte pieces in an
-// order that depends on the row, so that writes, row and column reads all spread over the banks (DecTile).  The next chunk's
-// rows are fetched into registers while the present one is computed.
+// order that depends on the row, so that writes, row and column reads all spread over the banks (DecTile; conflict cycles
+// counted per LDS instruction: none in the states' kernel of bf16, 1.8-1.9 in the outputs', 2.5 in f32).  The next chunk's rows
+// are fetched into registers while the present one is computed.
 //
-// What bounds it: the chain of a chunk (stage, two products, the state's update between two barriers), 1.5 us for 64 frames when
-// a workgroup has a CU to itself, 2.3 us when two share it; uniform batches of bf16 run at 4.2-4.5 TB/s, where a large copy does
-// 4.75.  Heads of 64, lengths from a tenth of the frames up: 64 x 400 x 6 bf16 16.6 us forward, 32.8 us backward; 32 x 3000 x 6
-// 76 and 112 us (the longest utterance's 47 chunks); one utterance of 23999 frames 38 us in 125 segments (states 12, join 7,
-// outputs 19); 16 x 400 x 6 f32 9 + 18 and 44 us: 13 chunks of 32 frames in the chain, 3.3 us each, 1.5 us of them the
-// exact-f32 products of one SIMD.
+// What bounds it: the chain of a chunk (stage, two products, the state's update between two barriers), 1.7 us for 64 frames when
+// a workgroup has a CU to itself, 2.6-2.9 us when two share it.  Batches of full length, bf16: 128 x 400 x 6 heads of 64 36 us,
+// 4.3 TB/s; 64 x 3000 x 6 171 us, 3.4 TB/s (a large copy: 4.76).  Lengths from a tenth of the frames up: 64 x 400 x 6 bf16 18.8 us
+// forward, 38 us backward; 32 x 3000 x 6 29 + 58 and 124 us; one utterance of 23999 frames 39 us in 75 segments (states 12, join
+// 5.5, outputs 21); 16 x 400 x 6 f32 9.6 + 17.5 and 44 us: 13 chunks of 32 frames in the chain, 3.3 us each, of which a SIMD's
+// exact-f32 products are 2800 cycles (64 operations a cycle), 1.2 us.
 //
 // Rounding: products accumulate in 32 bits and the state is held in 32 bits.  bf16 tensors: P and the copy of S that multiplies
 // q enter their products in two bf16 terms each, so 2^-16 of a value is lost: an output may hang on a single P, at the start of
